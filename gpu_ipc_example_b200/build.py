@@ -31,6 +31,8 @@ CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 LL_OPS = ["ArParallel", "ArSequential", "ArRing", "ArBisect", "ArOneShot", "AgRing", "AgDirect", "RsParallel"]
 LL_TYPES = {"f16": "__half", "bf16": "__nv_bfloat16"}
 
+PAGED_UNITS = ["model/paged_tables.cu", "model/paged_append.cu", "model/paged_attention.cu", "model/verify_drafts.cu"]
+
 ARCH = "-gencode arch=compute_100a,code=sm_100a"
 
 
@@ -116,6 +118,8 @@ def ninja_text(with_torch: bool = True) -> str:
     core_objs.append(cu("fused/gemm_local.cu"))
     core_objs.append(cu("model/decode_ops.cu"))
     core_objs.append(cu("model/decode_step.cu"))
+    for src in PAGED_UNITS:
+        core_objs.append(cu(src))
 
     lib = f"{PKG}/libb200ipc.so"
     w(f"build {lib}: link_so {' '.join(core_objs)}")
@@ -171,7 +175,7 @@ def cuda_units():
     """(source, extra flags) of every CUDA translation unit of the library."""
     units = [("coll/ll_inst.cu", f"-DB200_LL_OP={op} -DB200_LL_T={ty}") for op in LL_OPS for ty in LL_TYPES.values()]
     units += [(src, "") for src in ("coll/bulk_inst.cu", "fused/fused_ops.cu", "fused/gemm_ar.cu", "fused/gemm_local.cu", "model/decode_ops.cu", "model/decode_step.cu",
-                                    "capi/no_alloc.cu")]
+                                    "capi/no_alloc.cu", *PAGED_UNITS)]
     return units
 
 

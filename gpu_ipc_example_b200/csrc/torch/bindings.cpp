@@ -34,6 +34,7 @@
 #include "../fused/fused_ops.h"
 #include "../model/decode_ops.h"
 #include "../model/decode_step.h"
+#include "../model/paged_ops.h"
 
 namespace {
 
@@ -686,6 +687,169 @@ at::Tensor silu_mul_op(at::Tensor gate_up) {
   return act;
 }
 
+// ---- paged serving (model/paged_ops.h) ------------------------------------------------------------------
+// What is wrong with the arguments is said before anything is looked for on a GPU.
+void check_ints(const at::Tensor& t, at::ScalarType type, at::IntArrayRef sizes, const char* op, const char* what) {
+  TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.sizes() == sizes, "b200ipc: ", op, ": ", what, " must be a contiguous ", type,
+              " tensor of shape ", sizes, ", got ", t.scalar_type(), " ", t.sizes());
+}
+void check_one_device(std::initializer_list<const at::Tensor*> ts, const char* op) {
+  const at::Device d = (*ts.begin())->device();
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(t->is_cuda() && t->device() == d, "b200ipc: ", op, " takes tensors of one CUDA device, got ", t->device(), " beside ", d);
+}
+void check_apart(const at::Tensor& a, const at::Tensor& b, const char* op) {
+  if (a.nbytes() == 0 || b.nbytes() == 0) return;
+  const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
+  TORCH_CHECK(pa + a.nbytes() <= pb || pb + b.nbytes() <= pa, "b200ipc: ", op, ": tensors that are written must not overlap others");
+}
+void check_paged_table(const at::Tensor& table, const at::Tensor& lens, int64_t page, const char* op) {
+  TORCH_CHECK(table.dim() == 2 && table.size(0) >= 1 && table.size(0) <= kPagedMaxRequests && table.size(1) >= 1 && table.size(1) <= (1 << 27), "b200ipc: ", op,
+              ": the block table must be [requests, width], 1 to ", kPagedMaxRequests, " requests, got ", table.sizes());
+  TORCH_CHECK(page >= 1 && page <= (1 << 20), "b200ipc: ", op, ": bad page size ", page);
+  check_ints(table, at::kInt, table.sizes(), op, "the block table");
+  check_ints(lens, at::kInt, {table.size(0)}, op, "lens");
+}
+
+// (cu_new [B + 1], slots [rows], positions [rows], status [1])
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_extend_op(at::Tensor table, at::Tensor lens, at::Tensor new_lens, at::Tensor free_pages,
+                                                                           at::Tensor n_free, int64_t page, int64_t rows) {
+  constexpr const char* op = "paged_extend";
+  check_paged_table(table, lens, page, op);
+  const int64_t B = table.size(0);
+  check_ints(new_lens, at::kInt, {B}, op, "new_lens");
+  TORCH_CHECK(free_pages.dim() == 1, "b200ipc: paged_extend: free_pages must be a vector");
+  check_ints(free_pages, at::kInt, free_pages.sizes(), op, "free_pages");
+  check_ints(n_free, at::kInt, {1}, op, "n_free");
+  TORCH_CHECK(rows >= 0 && rows <= (int64_t(1) << 30) && free_pages.numel() <= (int64_t(1) << 30), "b200ipc: paged_extend: bad number of rows or pages");
+  check_one_device({&table, &lens, &new_lens, &free_pages, &n_free}, op);
+  for (const at::Tensor* w : {&table, &lens, &n_free}) {
+    for (const at::Tensor* t : {&table, &lens, &new_lens, &free_pages, &n_free})
+      if (t != w) check_apart(*w, *t, op);
+  }
+  c10::cuda::CUDAGuard guard(table.device());
+  at::Tensor cu = at::empty({B + 1}, table.options()), slots = at::empty({rows}, table.options().dtype(at::kLong)),
+             positions = at::empty({rows}, table.options()), status = at::empty({1}, table.options());
+  paged_extend(table.data_ptr<int>(), lens.data_ptr<int>(), new_lens.data_ptr<int>(), free_pages.data_ptr<int>(), n_free.data_ptr<int>(),
+               cu.data_ptr<int>(), slots.data_ptr<int64_t>(), positions.data_ptr<int>(), status.data_ptr<int>(), int(B), int(table.size(1)),
+               int(free_pages.numel()), int(page), int(rows), at::cuda::getCurrentCUDAStream(table.get_device()));
+  return {cu, slots, positions, status};
+}
+
+at::Tensor paged_trim_op(at::Tensor table, at::Tensor lens, at::Tensor keep_lens, at::Tensor free_pages, at::Tensor n_free, int64_t page) {
+  constexpr const char* op = "paged_trim";
+  check_paged_table(table, lens, page, op);
+  check_ints(keep_lens, at::kInt, {table.size(0)}, op, "keep_lens");
+  TORCH_CHECK(free_pages.dim() == 1 && free_pages.numel() <= (int64_t(1) << 30), "b200ipc: paged_trim: free_pages must be a vector");
+  check_ints(free_pages, at::kInt, free_pages.sizes(), op, "free_pages");
+  check_ints(n_free, at::kInt, {1}, op, "n_free");
+  check_one_device({&table, &lens, &keep_lens, &free_pages, &n_free}, op);
+  for (const at::Tensor* w : {&table, &lens, &free_pages, &n_free}) {
+    for (const at::Tensor* t : {&table, &lens, &keep_lens, &free_pages, &n_free})
+      if (t != w) check_apart(*w, *t, op);
+  }
+  c10::cuda::CUDAGuard guard(table.device());
+  at::Tensor status = at::empty({1}, table.options());
+  paged_trim(table.data_ptr<int>(), lens.data_ptr<int>(), keep_lens.data_ptr<int>(), free_pages.data_ptr<int>(), n_free.data_ptr<int>(),
+             status.data_ptr<int>(), int(table.size(0)), int(table.size(1)), int(free_pages.numel()), int(page),
+             at::cuda::getCurrentCUDAStream(table.get_device()));
+  return status;
+}
+
+// The caches [pages, hkv, page, 128] and rows [rows, >= columns] of 16-bit values, 16-byte aligned rows (the columns may be part of wider rows).
+void check_paged_cache(const at::Tensor& rows, int64_t columns, const at::Tensor& k, const at::Tensor& v, int64_t hq, int64_t hkv, const char* op) {
+  TORCH_CHECK(hq >= 1 && hkv >= 1 && hq % hkv == 0 && hq <= 65536, "b200ipc: ", op, ": the query heads must be a multiple of the KV heads, got ", hq, " and ", hkv);
+  dtype_of(rows);
+  TORCH_CHECK(k.dim() == 4 && k.size(1) == hkv && k.size(3) == 128 && v.sizes() == k.sizes() && k.is_contiguous() && v.is_contiguous() &&
+                  k.scalar_type() == rows.scalar_type() && v.scalar_type() == rows.scalar_type(),
+              "b200ipc: ", op, ": the caches must be contiguous [pages, ", hkv, ", page, 128] of the rows' type, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(k.size(0) >= 1 && k.size(2) >= 1 && k.numel() / 128 < (int64_t(1) << 31), "b200ipc: ", op, ": a cache of no pages, or of more than 2^31 rows");
+  TORCH_CHECK(rows.dim() == 2 && rows.size(1) >= columns && rows.stride(1) == 1 && (rows.size(0) <= 1 || rows.stride(0) >= columns) && rows.size(0) < (int64_t(1) << 30),
+              "b200ipc: ", op, " takes rows of at least ", columns, " contiguous elements, got ", rows.sizes(), " with strides ", rows.strides());
+  for (const at::Tensor* t : {&rows, &k, &v})
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0 && (t != &rows || rows.size(0) <= 1 || rows.stride(0) % 8 == 0), "b200ipc: ", op,
+                ": rows and caches must be 16-byte aligned");
+}
+
+at::Tensor rope_paged_append_op(at::Tensor qkv, at::Tensor kcache, at::Tensor vcache, at::Tensor slots, at::Tensor positions, int64_t hq, int64_t hkv,
+                                double theta) {
+  constexpr const char* op = "rope_paged_append";
+  check_paged_cache(qkv, (hq + 2 * hkv) * 128, kcache, vcache, hq, hkv, op);
+  check_ints(slots, at::kLong, {qkv.size(0)}, op, "slots");
+  check_ints(positions, at::kInt, {qkv.size(0)}, op, "positions");
+  TORCH_CHECK(theta > 0 && std::isfinite(theta), "b200ipc: rope_paged_append: theta must be a positive number");
+  check_one_device({&qkv, &kcache, &vcache, &slots, &positions}, op);
+  check_apart(kcache, vcache, op);
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor q = at::empty({qkv.size(0), hq * 128}, qkv.options());
+  rope_paged_append(dtype_of(qkv), qkv.data_ptr(), qkv.stride(0), q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), slots.data_ptr<int64_t>(),
+                    positions.data_ptr<int>(), int(qkv.size(0)), int(hq), int(hkv), int(kcache.size(2)), kcache.size(0), theta,
+                    at::cuda::getCurrentCUDAStream(qkv.get_device()));
+  return q;
+}
+
+int64_t paged_workspace_bytes(int64_t group, int64_t max_new, int64_t device) {
+  TORCH_CHECK(group >= 1 && group <= 65536 && max_new >= 1 && max_new < (int64_t(1) << 30), "b200ipc: paged_attention: bad number of heads or tokens");
+  return int64_t(paged_attention_workspace_bytes(int(group), int(max_new), sm_count_of(int(device))));
+}
+
+at::Tensor paged_attention_op(at::Tensor q, at::Tensor kcache, at::Tensor vcache, at::Tensor table, at::Tensor lens, at::Tensor cu_new, at::Tensor workspace,
+                              int64_t hq, int64_t hkv, int64_t max_new) {
+  constexpr const char* op = "paged_attention";
+  check_paged_cache(q, hq * 128, kcache, vcache, hq, hkv, op);
+  const int64_t page = kcache.size(2);
+  check_paged_table(table, lens, page, op);
+  check_ints(cu_new, at::kInt, {table.size(0) + 1}, op, "cu_new");
+  TORCH_CHECK(page == 16 || page == 32 || page == 64 || page == 128, "b200ipc: paged_attention: pages of 16, 32, 64 or 128 positions, got ", page);
+  TORCH_CHECK(table.size(1) * page < (int64_t(1) << 30), "b200ipc: paged_attention: a request of 2^30 positions or more");
+  TORCH_CHECK(max_new >= 1 && max_new < (int64_t(1) << 30), "b200ipc: paged_attention: max_new must be at least 1, got ", max_new);
+  TORCH_CHECK(hq / hkv <= 64, "b200ipc: paged_attention: at most 64 query heads per KV head, got ", hq / hkv);
+  TORCH_CHECK(q.size(0) * (hq / hkv) < (int64_t(1) << 30), "b200ipc: paged_attention: too many rows");
+  check_one_device({&q, &kcache, &vcache, &table, &lens, &cu_new, &workspace}, op);
+  TORCH_CHECK(workspace.is_contiguous() && int64_t(workspace.nbytes()) >= paged_workspace_bytes(hq / hkv, max_new, q.get_device()) &&
+                  (reinterpret_cast<uintptr_t>(workspace.data_ptr()) & 255) == 0,
+              "b200ipc: paged_attention workspace too small or not 256-byte aligned");
+  for (const at::Tensor* t : {&q, &kcache, &vcache, &table, &lens, &cu_new}) check_apart(workspace, *t, op);
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty({q.size(0), hq * 128}, q.options());
+  if (q.size(0) == 0) return out;
+  const PagedAttentionShape s{int(q.size(0)), int(table.size(0)), int(hq), int(hkv), int(page), int(table.size(1)), kcache.size(0), int(std::min(max_new, q.size(0)))};
+  paged_attention(dtype_of(q), q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), table.data_ptr<int>(), lens.data_ptr<int>(),
+                  cu_new.data_ptr<int>(), out.data_ptr(), workspace.data_ptr(), s, sm_count_of(q.get_device()), at::cuda::getCurrentCUDAStream(q.get_device()));
+  return out;
+}
+
+// (tokens [B, K + 1], accepted [B])
+std::tuple<at::Tensor, at::Tensor> verify_drafts_op(at::Tensor target, const std::optional<at::Tensor>& draft, at::Tensor tokens,
+                                                    const std::optional<at::Tensor>& draft_lens, at::Tensor accept, at::Tensor sample) {
+  constexpr const char* op = "verify_drafts";
+  TORCH_CHECK(tokens.dim() == 2 && tokens.size(1) <= 1024 && tokens.size(0) < (1 << 24), "b200ipc: verify_drafts: draft_tokens must be [requests, drafts], at most 1024 drafts");
+  const int64_t B = tokens.size(0), K = tokens.size(1);
+  check_ints(tokens, at::kLong, {B, K}, op, "draft_tokens");
+  check_ints(accept, at::kFloat, {B, K}, op, "accept");
+  check_ints(sample, at::kFloat, {B}, op, "sample");
+  if (draft_lens) check_ints(*draft_lens, at::kInt, {B}, op, "draft_lens");
+  TORCH_CHECK(target.dim() == 3 && target.size(0) == B && target.size(1) == K + 1 && target.size(2) >= 1 && target.scalar_type() == at::kFloat &&
+                  (target.stride(2) == 1 || target.size(2) == 1),
+              "b200ipc: verify_drafts: target_probs must be float32 [", B, ", ", K + 1, ", words] with contiguous words, got ", target.sizes());
+  const int64_t V = target.size(2);
+  TORCH_CHECK(V < (int64_t(1) << 31), "b200ipc: verify_drafts: too many words");
+  if (draft)
+    TORCH_CHECK(draft->dim() == 3 && draft->size(0) == B && draft->size(1) == K && draft->size(2) == V && draft->scalar_type() == at::kFloat &&
+                    (draft->stride(2) == 1 || V == 1),
+                "b200ipc: verify_drafts: draft_probs must be float32 [", B, ", ", K, ", ", V, "] with contiguous words, got ", draft->sizes());
+  check_one_device({&target, &tokens, &accept, &sample}, op);
+  if (draft) check_one_device({&target, &*draft}, op);
+  if (draft_lens) check_one_device({&target, &*draft_lens}, op);
+  c10::cuda::CUDAGuard guard(target.device());
+  at::Tensor out = at::empty({B, K + 1}, tokens.options()), accepted = at::empty({B}, tokens.options().dtype(at::kInt));
+  const VerifyShape s{int(B), int(K), V, target.stride(0), target.stride(1), draft ? draft->stride(0) : 0, draft ? draft->stride(1) : 0};
+  verify_drafts(target.data_ptr<float>(), draft ? draft->data_ptr<float>() : nullptr, tokens.data_ptr<int64_t>(),
+                draft_lens ? draft_lens->data_ptr<int>() : nullptr, accept.data_ptr<float>(), sample.data_ptr<float>(), out.data_ptr<int64_t>(),
+                accepted.data_ptr<int>(), s, at::cuda::getCurrentCUDAStream(target.get_device()));
+  return {out, accepted};
+}
+
 // ---- the list calls of Communicator, past the dispatcher -----------------------------------------------------------------
 // A small collective is bound by its call: through torch.ops the lists of an 8-rank world cost about 7 us before the launch,
 // as CPython calls 2.  A call comes this way only where nothing listens on the way there and its tensors are plain ones: no
@@ -942,6 +1106,16 @@ TORCH_LIBRARY(b200ipc, m) {
   m.def("decode_step(Tensor(a!) h, Tensor[] wqkv, Tensor[] wo, Tensor[] wgu, Tensor[] wdown, Tensor(b!)[] kcache, Tensor(c!)[] vcache, Tensor[] head, "
         "Tensor[] gamma_attn, Tensor[] gamma_mlp, Tensor gamma_final, Tensor(d!) workspace, int hq, int hkv, int pos, float eps, float theta, "
         "int comm, int flags=0) -> Tensor[]", &decode_step_op);
+  m.def("paged_extend(Tensor(a!) block_table, Tensor(b!) lens, Tensor new_lens, Tensor free_pages, Tensor(c!) n_free, int page, int rows) -> "
+        "(Tensor, Tensor, Tensor, Tensor)", &paged_extend_op);
+  m.def("paged_trim(Tensor(a!) block_table, Tensor(b!) lens, Tensor keep_lens, Tensor(c!) free_pages, Tensor(d!) n_free, int page) -> Tensor",
+        &paged_trim_op);
+  m.def("rope_paged_append(Tensor qkv, Tensor(a!) kcache, Tensor(b!) vcache, Tensor slots, Tensor positions, int hq, int hkv, float theta) -> Tensor",
+        &rope_paged_append_op);
+  m.def("paged_attention(Tensor q, Tensor kcache, Tensor vcache, Tensor block_table, Tensor lens, Tensor cu_new, Tensor(a!) workspace, int hq, "
+        "int hkv, int max_new) -> Tensor", &paged_attention_op);
+  m.def("verify_drafts(Tensor target_probs, Tensor? draft_probs, Tensor draft_tokens, Tensor? draft_lens, Tensor accept, Tensor sample) -> "
+        "(Tensor, Tensor)", &verify_drafts_op);
   m.def("rmsnorm(Tensor x, Tensor gamma, float eps) -> Tensor", &rmsnorm_op);
   m.def("row_argmax(Tensor x) -> (Tensor, Tensor)", &row_argmax_op);
   m.def("silu_mul(Tensor gate_up) -> Tensor", &silu_mul_op);
@@ -996,6 +1170,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("gemm_ar_workspace_bytes", &gemm_ar_workspace_bytes);
   m.def("decode_step_workspace_bytes", &step_workspace_bytes);
+  m.def("paged_attention_workspace_bytes", &paged_workspace_bytes);
   m.def("attention_splits", &attention_splits);
   m.def("attention_workspace_bytes", &attention_workspace_bytes);
   m.def("algo_names", &algo_names_help);
