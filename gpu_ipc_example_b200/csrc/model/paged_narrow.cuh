@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           }
           if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
             const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
-            const float ca = na == -INFINITY ? 1.f : exp2f(ma - na), cb = nb == -INFINITY ? 1.f : exp2f(mb - nb);
+            const float ca = na == -INFINITY ? 1.f : exp2_fast(ma - na), cb = nb == -INFINITY ? 1.f : exp2_fast(mb - nb);
             ma = na;
             mb = nb;
             sa *= ca;
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           uint32_t pw[4];  // the weights as the next product's left operand
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float p0 = exp2f(s[j][0] - ua), p1 = exp2f(s[j][1] - ua), p2 = exp2f(s[j][2] - ub), p3 = exp2f(s[j][3] - ub);
+            const float p0 = exp2_fast(s[j][0] - ua), p1 = exp2_fast(s[j][1] - ua), p2 = exp2_fast(s[j][2] - ub), p3 = exp2_fast(s[j][3] - ub);
             sa += p0 + p1;
             sb += p2 + p3;
             pw[2 * j] = pack2<T>(p0, p1);
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           const float2 a = s_ml[w4][r8], b = s_ml[w4][r8 + 8];
           const float na = fmaxf(ma, a.x), nb = fmaxf(mb, b.x);
           const float ua = na == -INFINITY ? 0.f : na, ub = nb == -INFINITY ? 0.f : nb;
-          const float fa = exp2f(ma - ua), fb = exp2f(mb - ub), ga = exp2f(a.x - ua), gb = exp2f(b.x - ub);
+          const float fa = exp2_fast(ma - ua), fb = exp2_fast(mb - ub), ga = exp2_fast(a.x - ua), gb = exp2_fast(b.x - ub);
           ma = na;
           mb = nb;
           sa = sa * fa + a.y * ga;
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
         float4 v = make_float4(0, 0, 0, 0);
         for (int s = 0; s < slices; ++s) {
           const float2 ml = s_ml[s * blocks + b][in];
-          const float f = exp2f(ml.x - u);
+          const float f = exp2_fast(ml.x - u);
           const float4 x = *reinterpret_cast<const float4*>(s_o + ((s * blocks + b) * 16 + in) * kNarORow + lane * 4);
           l += ml.y * f;
           v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
@@ -326,11 +326,12 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   if (threadIdx.x == 0 && *abort_flag) *args.status = 1;
 }
 
+constexpr int kNarJoin = 8;  // warps of a row: one request alone leaves a piece on every SM
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_narrow_join_kernel(const __grid_constant__ PagedArgs args, int spans) {
   pdl_launch_dependents();
   pdl_wait();
-  join_row<T, kNarRows>(args, spans, int(blockIdx.x), int(blockIdx.y), [&](const int4& item, int row) -> T* {
+  join_rows<T, kNarRows, kNarJoin>(args, spans, [&](const int4& item, int row) -> T* {
     const Request r = request_at(args, item.x);
     if (row >= r.n * args.group) return nullptr;
     const int j = row / args.group;

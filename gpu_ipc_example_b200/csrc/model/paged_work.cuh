@@ -37,6 +37,13 @@ struct PagedArgs {
   float scale_log2;
 };
 
+// 2^x in one instruction: relative error 2^-22, results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct Request {
   int row0, n, len;  // first row of q, new tokens, tokens in the cache
 };
@@ -140,19 +147,21 @@ __device__ __forceinline__ void lead(const PagedArgs& a) {
 }
 
 // ---- the join ---------------------------------------------------------------------------------------------------------
-// One CTA per span and row of a piece: where an item starts in this span and goes on in the next, its pieces are weighted with
-// 2^(maximum - greatest maximum) and added in order.  Eight warps take every eighth piece each.  `locate(item, row)`: the output row.
+// Where an item starts in span c and goes on in the next, its pieces are weighted with 2^(maximum - greatest maximum) and added in order.  A
+// row is WARPS warps' work, each takes every WARPS-th piece; kJoinThreads / 32 / WARPS rows a CTA, span blockIdx.x.  `locate(item, row)`: the output row.
 constexpr int kJoinThreads = 256;
-template <typename T, int ROWS, typename Locate>
-__device__ __forceinline__ void join_row(const PagedArgs& a, int spans, int c, int row, Locate locate) {
+template <typename T, int ROWS, int WARPS, typename Locate>
+__device__ __forceinline__ void join_rows(const PagedArgs& a, int spans, Locate locate) {
   constexpr int kWarps = kJoinThreads / 32;
   __shared__ float s_m[kWarps], s_l[kWarps];
   __shared__ __align__(16) float4 s_o[kWarps][32];
+  const int c = int(blockIdx.x);
   const int4 here = a.starts[c], next = a.starts[c + 1];
   if (next.z == 0 || (here.x == next.x && here.y == next.y && here.z > 0)) return;  // nothing starts here that goes on
-  T* dst = locate(next, row);
-  if (dst == nullptr) return;
   const int warp = int(threadIdx.x >> 5), lane = int(threadIdx.x & 31);
+  const int row = int(blockIdx.y) * (kWarps / WARPS) + warp / WARPS;
+  T* dst = locate(next, row);
+  if (__syncthreads_count(dst != nullptr) == 0) return;
   int pieces = 1;  // and one in each of the following spans that start inside of the item
   for (int k0 = c + 1; k0 < spans; k0 += kJoinThreads) {
     const int k = k0 + int(threadIdx.x);
@@ -161,16 +170,18 @@ __device__ __forceinline__ void join_row(const PagedArgs& a, int spans, int c, i
   }
   float m = -INFINITY, l = 0;
   float4 o = make_float4(0, 0, 0, 0);
+  if (dst != nullptr) {
 #pragma unroll 4
-  for (int n = warp; n < pieces; n += kWarps) {
-    const float* p = Piece<ROWS>::slot(a, c + n, n == 0 ? 1 : 0);
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + 2 * row));
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + size_t(row) * kAttnD + lane * 4));
-    const float mn = fmaxf(m, ml.x), u = mn == -INFINITY ? 0.f : mn;
-    const float c0 = exp2f(m - u), c1 = exp2f(ml.x - u);
-    m = mn;
-    l = l * c0 + ml.y * c1;
-    o = make_float4(o.x * c0 + v.x * c1, o.y * c0 + v.y * c1, o.z * c0 + v.z * c1, o.w * c0 + v.w * c1);
+    for (int n = warp % WARPS; n < pieces; n += WARPS) {
+      const float* p = Piece<ROWS>::slot(a, c + n, n == 0 ? 1 : 0);
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + 2 * row));
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + size_t(row) * kAttnD + lane * 4));
+      const float mn = fmaxf(m, ml.x), u = mn == -INFINITY ? 0.f : mn;
+      const float c0 = exp2_fast(m - u), c1 = exp2_fast(ml.x - u);
+      m = mn;
+      l = l * c0 + ml.y * c1;
+      o = make_float4(o.x * c0 + v.x * c1, o.y * c0 + v.y * c1, o.z * c0 + v.z * c1, o.w * c0 + v.w * c1);
+    }
   }
   if (lane == 0) {
     s_m[warp] = m;
@@ -178,20 +189,19 @@ __device__ __forceinline__ void join_row(const PagedArgs& a, int spans, int c, i
   }
   s_o[warp][lane] = o;
   __syncthreads();
-  if (warp == 0) {
+  if (warp % WARPS == 0 && dst != nullptr) {
     m = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w]);
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_m[warp + w]);
     l = 0;
     o = make_float4(0, 0, 0, 0);
-    for (int w = 0; w < kWarps; ++w) {
-      const float x = s_m[w] == -INFINITY ? 0.f : exp2f(s_m[w] - m);
-      const float4 v = s_o[w][lane];
-      l += s_l[w] * x;
+    for (int w = 0; w < WARPS; ++w) {
+      const float x = s_m[warp + w] == -INFINITY ? 0.f : exp2_fast(s_m[warp + w] - m);
+      const float4 v = s_o[warp + w][lane];
+      l += s_l[warp + w] * x;
       o = make_float4(o.x + v.x * x, o.y + v.y * x, o.z + v.z * x, o.w + v.w * x);
     }
     const float inv = l == 0 ? 0.f : 1 / l;
-    const uint2 packed{pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv)};
-    *reinterpret_cast<uint2*>(dst + lane * 4) = packed;
+    *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
   }
 }
 
