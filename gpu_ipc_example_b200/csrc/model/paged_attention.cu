@@ -19,22 +19,36 @@ CUtensorMap cache_map(DType t, const void* cache, const PagedAttentionShape& s) 
   return map;
 }
 
+// Q so that 128 rows of an item, heads of a group side by side, are one box for each half of the dimensions.
+CUtensorMap query_map(DType t, const PagedArgs& a) {
+  CUtensorMap map;
+  const cuuint64_t head = kAttnD * 2, stride = a.rows > 1 ? cuuint64_t(a.row_stride) * 2 : cuuint64_t(a.hq) * head;
+  cuuint64_t dims[5] = {64, 2, cuuint64_t(a.group), cuuint64_t(a.hkv), cuuint64_t(a.rows)};
+  cuuint64_t strides[4] = {128, head, head * cuuint64_t(a.group), stride};
+  cuuint32_t box[5] = {64, 1, cuuint32_t(a.group), 1, cuuint32_t(128 / a.group)}, one[5] = {1, 1, 1, 1, 1};
+  B200_CU_CHECK(cu().TensorMapEncodeTiled(&map, t == DType::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+                                          const_cast<void*>(a.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
+  return map;
+}
+
 // The workspace: a status word, then for each kernel where the spans start, then the pieces.
 constexpr size_t kHead = 256;
 size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
-size_t starts_bytes(int spans) { return round_up(size_t(spans + 1) * sizeof(int4)); }
+size_t starts_bytes(int spans) { return round_up(size_t(spans + 1) * sizeof(Start)); }
 template <int ROWS>
 size_t pieces_bytes(int spans) { return round_up(size_t(spans) * 2 * Piece<ROWS>::kFloats * sizeof(float)); }
 
 // A kernel over the spans, and the one that joins its pieces.
-template <int ROWS>
-void launch_pair(const void* kernel, int threads, size_t smem, const void* join, unsigned join_rows, PagedArgs& a, int spans, char* workspace, cudaStream_t stream) {
-  a.starts = reinterpret_cast<int4*>(workspace);
+template <typename T, int ROWS>
+void launch_pair(const void* kernel, int threads, size_t smem, PagedArgs& a, int spans, char* workspace, int64_t most_rows, cudaStream_t stream) {
+  a.starts = reinterpret_cast<Start*>(workspace);
   a.part = reinterpret_cast<float*>(workspace + starts_bytes(spans));
   B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
   void* params[] = {&a, &spans};
   B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(unsigned(threads)), params, smem, stream, true));
-  B200_CUDA_CHECK(launch_maybe_pdl(join, dim3(unsigned(spans), join_rows), dim3(kJoinThreads), params, 0, stream, true));
+  const unsigned groups = unsigned((std::min<int64_t>(most_rows, ROWS) + kJoinRows - 1) / kJoinRows);
+  B200_CUDA_CHECK(launch_maybe_pdl(reinterpret_cast<const void*>(&paged_join_kernel<T, ROWS>), dim3(unsigned(spans), groups), dim3(kJoinThreads), params, 0, stream, true));
 }
 
 template <typename T>
@@ -45,15 +59,15 @@ void run(PagedArgs& a, const PagedAttentionShape& s, char* workspace, int spans,
   a.narrow_rows = narrow ? kNarRows : 0;
   a.leads = 1;
   if (narrow) {
-    const unsigned rows = unsigned(std::min<int64_t>(most, kNarRows));
-    launch_pair<kNarRows>(reinterpret_cast<const void*>(&paged_narrow_kernel<T>), kNarThreads, kNarSmem, reinterpret_cast<const void*>(&paged_narrow_join_kernel<T>),
-                          rows, a, spans, workspace, stream);
+    launch_pair<T, kNarRows>(reinterpret_cast<const void*>(&paged_narrow_kernel<T>), kNarThreads, kNarSmem, a, spans, workspace, most, stream);
     workspace += starts_bytes(spans) + pieces_bytes<kNarRows>(spans);
     a.leads = 0;
   }
-  if (wide)
-    launch_pair<kWideRows>(reinterpret_cast<const void*>(&paged_wide_kernel<T>), kWideThreads, kWideSmem, reinterpret_cast<const void*>(&paged_wide_join_kernel<T>),
-                           unsigned(kWideRows * kWideJoin / (kJoinThreads / 32)), a, spans, workspace, stream);
+  if (wide) {
+    a.q_boxes = 128 % a.group == 0;
+    if (a.q_boxes) a.tma_q = query_map(std::is_same<T, __half>::value ? DType::F16 : DType::BF16, a);
+    launch_pair<T, kWideRows>(reinterpret_cast<const void*>(&paged_wide_kernel<T>), kWideThreads, kWideSmem, a, spans, workspace, most, stream);
+  }
 }
 
 }  // namespace

@@ -1,41 +1,47 @@
-// Attention over a paged cache for requests with few rows: up to 64 of (new tokens x query heads of a KV head).  Single tokens of a decoding
-// server, drafts behind them, short prompts.
+// Attention over a paged cache for requests with few rows: up to 16 of (new tokens x query heads of a KV head).  Single tokens of a
+// decoding server, a few drafts behind them.
 //
-// Bound by memory: every position of a request is 512 bytes of K and V per KV head and read once for all of the item's rows.  One thread
-// per box streams the pages by TMA (128-byte swizzle) into a ring of six stages of 64 positions, 192 KB in flight per SM; a page that the cache
-// does not have is a box outside of the tensor, which reads zeros.  Eight warps compute with mma.sync (m16n8k16): at most 64 rows
-// cannot fill tcgen05's 128, and its accumulators would have to be fetched back for every 64 positions.  Warps 0-3 take the tiles in even
-// stages, 4-7 those in odd ones (always the same stages: a wait for a stage's next round must come from who has seen the round before, as
-// copies may land out of order); of the four, as many share the rows as there are blocks of 16 rows (one, two or four) and the rest
-// splits the tile's positions.  Scores, maxima, sums and outputs are fp32; the weights are rounded to 16 bits for the second product, as the
-// tensor cores take them.
+// Bound by memory: every position of a request is 512 bytes of K and V per KV head and read once for all of the item's rows.  One warp
+// streams the pages by TMA (128-byte swizzle) into a ring of six stages of 64 positions, 192 KB in flight per SM; a page that the cache
+// does not have is a box outside of the tensor, which reads zeros.  Eight warps compute with mma.sync (m16n8k16): 16 rows cannot fill
+// tcgen05's 128.  Warps 0-3 take the tiles in even stages, 4-7 those in odd ones (always the same stages: a wait for a stage's next round
+// must come from who has seen the round before, as copies may land out of order), 16 positions of a tile each.  Scores, maxima, sums
+// and outputs are fp32; the weights are rounded to 16 bits for the second product, as the tensor cores take them.
 #pragma once
 
 #include "paged_work.cuh"
 
 namespace b200ipc {
 
-constexpr int kNarRows = 64;
+constexpr int kNarRows = 16;
 constexpr int kNarTile = 64;     // positions
 constexpr int kNarStages = 6;    // even: a stage belongs to one half of the warps
-constexpr int kNarWarps = 8;     // that compute
-constexpr int kNarThreads = (kNarWarps + 1) * 32;
+constexpr int kNarWarps = 8;     // that compute; then the stream's and the walking one
+constexpr int kNarThreads = (kNarWarps + 2) * 32;
 constexpr int kNarTileBytes = kNarTile * kAttnD * 2;  // of K or V
 constexpr int kNarORow = kAttnD + 4;                  // floats of a row of the merge buffer
-constexpr size_t kNarSmem = 1024 + size_t(kNarStages) * 2 * kNarTileBytes + size_t(4) * 16 * kNarORow * 4;
+constexpr size_t kNarSmem = 1024 + size_t(kNarStages) * 2 * kNarTileBytes + size_t(kNarWarps) * 8 * kNarORow * 4;
 constexpr int kNarStart = 1;     // what an item's start and end cost, in tiles
 constexpr int kNarLeast = 2;     // a span is at least so long: more than kNarStart, so that every cut leaves a tile on both sides
+
+struct NarrowItem {
+  int valid;
+  int request, h;       // KV head
+  int first, n, len;    // the request's first row of q, its new tokens, its tokens in the cache
+  int t0, t1, whole;    // tiles of positions; whether these are all
+};
 
 struct NarrowCut {
   const PagedArgs& a;
   __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0 && r.n * a.group <= a.narrow_rows; }
   __device__ __forceinline__ int tiles(const Request& r) const { return (r.len + kNarTile - 1) / kNarTile; }
   __device__ __forceinline__ int64_t length(const Request& r) const { return takes(r) ? int64_t(a.hkv) * (kNarStart + tiles(r)) : 0; }
-  __device__ __forceinline__ int4 place(const Mark& m) const {
-    if (m.request >= a.requests) return make_int4(a.requests, 0, 0, 0);
-    const int per = kNarStart + tiles(request_at(a, m.request));
-    const int h = int(m.offset / per);
-    return make_int4(m.request, h, max(0, int(m.offset - int64_t(h) * per) - kNarStart), 0);
+  __device__ __forceinline__ Start place(const Mark& m) const {
+    if (m.request >= a.requests) return Start{a.requests, 0, 0, 0, 0, 0, 0};
+    const Request r = request_at(a, m.request);
+    const int per = kNarStart + tiles(r);
+    const int h = int(divide(m.offset, per));
+    return Start{m.request, h, max(0, int(m.offset - int64_t(h) * per) - kNarStart), r.n * a.group, int64_t(r.row0) * a.hq + h * a.group, 0, 0};
   }
 };
 
@@ -50,12 +56,13 @@ __device__ __forceinline__ void nar_sync() { asm volatile("bar.sync 1, %0;" ::"n
 template <typename T>
 __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __grid_constant__ PagedArgs args) {
   extern __shared__ unsigned char smem_raw[];
+  using Items = Queue<NarrowItem, kNarWarps + 1>;
+  __shared__ Items s_queue;
   __shared__ uint64_t full[kNarStages], empty[kNarStages];
-  __shared__ Mark s_marks[2];
   __shared__ int s_abort;
-  __shared__ float2 s_ml[4][16];
+  __shared__ float2 s_ml[kNarWarps][8];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_o = reinterpret_cast<float*>(ring + kNarStages * 2 * kNarTileBytes);  // [4][16][kNarORow]
+  float* s_o = reinterpret_cast<float*>(ring + kNarStages * 2 * kNarTileBytes);  // [8 warps][8 rows][kNarORow]
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = int(threadIdx.x & 31);
   volatile int* abort_flag = &s_abort;
   pdl_launch_dependents();
@@ -64,279 +71,259 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 4);
     }
+    s_queue.init();
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
+  reset_status(args);
   const NarrowCut cut{args};
-  find_span<kNarThreads>(args, [&](const Request& r) { return cut.length(r); }, kNarLeast, s_marks);
-  const int4 first = cut.place(s_marks[0]), last = cut.place(s_marks[1]);
-  if (threadIdx.x == 0) {
-    args.starts[blockIdx.x] = first;
-    if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
-  }
-  lead<T>(args);
-  const auto takes = [&](const Request& r) { return cut.takes(r); };
-  Window win;
+  Mark marks[2];
+  find_span<kNarThreads>(args, [&](const Request& r) { return cut.length(r); }, kNarLeast, warp == kNarWarps + 1, reinterpret_cast<int64_t*>(ring), marks);
+  QueueEnd<Items, NarrowItem> items{s_queue, abort_flag};
 
-  // Every role walks the items of the span alike: f(request, its number, head, first tile, tile behind the last, tiles of the item).
-  auto walk = [&](auto&& f) {
-    int i = first.x < args.requests ? win.next(args, first.x, takes) : args.requests, h = first.y, t0 = first.z;
-    while (i < args.requests && !(i > last.x || (i == last.x && (h > last.y || (h == last.y && t0 >= last.z))))) {
-      const Request r = win.get(i);
-      const int tiles = cut.tiles(r);
-      f(r, i, h, t0, i == last.x && h == last.y ? last.z : tiles, tiles);
-      t0 = 0;
-      if (++h == args.hkv) {
-        h = 0;
-        i = win.next(args, i + 1, takes);
+  if (warp == kNarWarps + 1) {
+    // ---- the walk ------------------------------------------------------------------------------------------------------------
+    const Start first = cut.place(marks[0]), last = cut.place(marks[1]);
+    if (lane == 0) {
+      args.starts[blockIdx.x] = first;
+      if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
+    }
+    const auto takes = [&](const Request& r) { return cut.takes(r); };
+    Window win;
+    int i = first.request < args.requests ? win.next(args, first.request, takes) : args.requests, h = first.number, t0 = first.tile;
+    for (bool more = true; more;) {
+      NarrowItem x{};
+      if (i < args.requests && !(i > last.request || (i == last.request && (h > last.number || (h == last.number && t0 >= last.tile))))) {
+        const Request r = win.get(i);
+        const int tiles = cut.tiles(r), t1 = i == last.request && h == last.number ? last.tile : tiles;
+        x = NarrowItem{1, i, h, r.row0, r.n, r.len, t0, t1, t0 == 0 && t1 == tiles};
+        t0 = 0;
+        if (++h == args.hkv) {
+          h = 0;
+          i = win.next(args, i + 1, takes);
+        }
       }
+      more = items.put(x);
     }
-  };
-
-  uint32_t st = 0, ph = 0;  // stage, and the parity of its round
-  auto step = [&]() {
-    if (++st == kNarStages) {
-      st = 0;
-      ph ^= 1u;
-    }
-  };
-  if (warp == kNarWarps) {
-    // ---- the stream: lane l loads box l / 4 of a tile, K or V, left or right half of the dimensions ----------------------
+  } else if (warp == kNarWarps) {
+    // ---- the stream: lane l knows where box l of a tile is; K and V, left and right half of the dimensions --------------------
     const int box = min(args.page, kNarTile), boxes = kNarTile / box, per_page = args.page / box;
-    const int sub = lane >> 2, half = lane & 1, value = (lane >> 1) & 1;
-    const int64_t outside = args.pages * args.hkv * args.page;
+    const int outside = int(args.pages * args.hkv * args.page);
+    uint32_t st = 0, ph = 0;
     int issued = 0;
-    walk([&](const Request& r, int i, int h, int t0, int t1, int) {
-      const int* table = args.table + int64_t(i) * args.width;
-      const int pages = (r.len + args.page - 1) / args.page;  // of the request
-      int base = -64, entry = 0;                              // 32 entries of its table, one per lane
-      for (int t = t0; t < t1; ++t) {
-        // every lane's box: which page, and where in it
-        const int b = t * boxes + sub, p = b / per_page, offset = (b - p * per_page) * box;
-        const int p_first = t * boxes / per_page;
-        if (p_first < base || (t * boxes + boxes - 1) / per_page >= base + 32) {
-          base = p_first;
+    for (const NarrowItem* x = items.take(); x != nullptr; x = items.take()) {
+      const int* table = args.table + int64_t(x->request) * args.width;
+      const int len = x->len, h = x->h, t1 = x->t1, pages = (len + args.page - 1) / args.page;
+      int base = -64, entry = 0;  // 32 entries of the request's table, one per lane
+      for (int t = x->t0; t < t1; ++t) {
+        const int b = t * boxes + (lane & (boxes - 1)), p = b / per_page;
+        if ((t * boxes + boxes - 1) / per_page >= base + 32) {
+          base = t * boxes / per_page;
           entry = base + lane < pages ? table[base + lane] : -1;
         }
-        const int64_t id = __shfl_sync(0xffffffffu, entry, min(31, p - base));
-        const int n = min(boxes, (r.len - t * kNarTile + box - 1) / box);  // boxes that hold positions of the request
-        mbar_wait_long(&empty[st], ph ^ 1u, abort_flag, kPagedTimeoutNs);
-        if (__any_sync(0xffffffffu, *abort_flag)) return;
+        const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
+        const int at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
+        const int n = min(boxes, (len - t * kNarTile + box - 1) / box);  // boxes that hold positions of the request
+        items.wait(&empty[st], ph ^ 1u);
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
         if (lane == 0) mbar_expect_tx(&full[st], uint32_t(n * box) * kAttnD * 4u);
         __syncwarp();
-        if (sub < n) {
-          const int row = int(id >= 0 && id < args.pages ? (id * args.hkv + h) * args.page + offset : outside);
-          unsigned char* dst = ring + st * 2 * kNarTileBytes + value * kNarTileBytes + half * (kNarTileBytes / 2) + sub * box * 128;
-          tma_load_2d(dst, value ? &args.tma_v : &args.tma_k, &full[st], half * 64, row);
+        unsigned char* dst = ring + st * 2 * kNarTileBytes;
+        for (int k = 0; k < n; ++k, dst += box * 128) {
+          const int row = __shfl_sync(0xffffffffu, at, k);
+          if (elect_one()) {
+            tma_load_2d(dst, &args.tma_k, &full[st], 0, row);
+            tma_load_2d(dst + kNarTileBytes / 2, &args.tma_k, &full[st], 64, row);
+            tma_load_2d(dst + kNarTileBytes, &args.tma_v, &full[st], 0, row);
+            tma_load_2d(dst + kNarTileBytes + kNarTileBytes / 2, &args.tma_v, &full[st], 64, row);
+          }
+          __syncwarp();
         }
         ++issued;
-        step();
+        if (++st == kNarStages) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
-    });
+      items.give_back();
+    }
     // copies in flight land before the CTA leaves
-    const uint64_t t0 = globaltimer_ns();
+    const uint64_t since = globaltimer_ns();
     for (int back = 1; back <= min(issued, kNarStages); ++back)
-      mbar_drain(&full[(issued - back) % kNarStages], uint32_t((issued - back) / kNarStages) & 1u, t0);
+      mbar_drain(&full[(issued - back) % kNarStages], uint32_t((issued - back) / kNarStages) & 1u, since);
   } else {
     // ---- the arithmetic ----------------------------------------------------------------------------------------------------
-    const int side = warp >> 2, w4 = warp & 3, r8 = lane >> 2, c = lane & 3, G = args.group;
+    const int side = warp >> 2, r8 = lane >> 2, c = lane & 3, G = args.group, at = (warp & 3) * 16;  // positions of a tile: at .. at + 15
     const uint32_t ring_addr = smem_u32(ring);
-    const uint32_t k_row = uint32_t(((lane >> 4) & 1) * 8 + (lane & 7)), k_chunk = (lane >> 3) & 1;
-    const uint32_t v_row = uint32_t(((lane >> 3) & 1) * 8 + (lane & 7)), v_chunk = (lane >> 4) & 1;
+    const uint32_t k_row = uint32_t(at + ((lane >> 4) & 1) * 8 + (lane & 7)), k_chunk = (lane >> 3) & 1;
+    const uint32_t v_row = uint32_t(at + ((lane >> 3) & 1) * 8 + (lane & 7)), v_chunk = (lane >> 4) & 1;
     auto chunk_addr = [](uint32_t tile, uint32_t pos, uint32_t chunk) {
       return tile + (chunk >> 3) * (kNarTileBytes / 2) + pos * 128 + (((chunk & 7) ^ (pos & 7)) << 4);
     };
-    walk([&](const Request& r, int, int h, int t0, int t1, int tiles) {
-      const bool odd_tiles = t1 - t0 > 1 || (t1 - t0 == 1 && (st & 1u));  // whether warps 4-7 have any
-      const int nrows = r.n * G, blocks = nrows <= 16 ? 1 : nrows <= 32 ? 2 : 4;
-      const int block = w4 & (blocks - 1), slice = blocks == 1 ? w4 : blocks == 2 ? w4 >> 1 : 0;
-      const int ra = block * 16 + r8, rb = ra + 8;  // this lane's two rows of the item
-      const int ja = ra / G, jb = rb / G;
-      auto row_of = [&](int row, int j) { return static_cast<const T*>(args.q) + int64_t(r.row0 + j) * args.row_stride + (int64_t(h) * G + (row - j * G)) * kAttnD; };
-      uint32_t qa[8][4];
-      {
-        const uint32_t *pa = reinterpret_cast<const uint32_t*>(row_of(ra, ja)), *pb = reinterpret_cast<const uint32_t*>(row_of(rb, jb));
+    uint32_t st = 0, ph = 0;
+    uint32_t qa[8][4];
+    // this lane's two rows of an item, r8 and r8 + 8
+    auto load_q = [&](const NarrowItem* x) {
+      const int nrows = x->n * G;
+      auto row_of = [&](int row) {
+        const int j = row / G;
+        return reinterpret_cast<const uint32_t*>(static_cast<const T*>(args.q) + int64_t(x->first + j) * args.row_stride + (int64_t(x->h) * G + (row - j * G)) * kAttnD);
+      };
+      const bool a = r8 < nrows, b = r8 + 8 < nrows;
+      const uint32_t *pa = row_of(a ? r8 : 0), *pb = row_of(b ? r8 + 8 : 0);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          qa[k][0] = ra < nrows ? pa[8 * k + c] : 0u;
-          qa[k][1] = rb < nrows ? pb[8 * k + c] : 0u;
-          qa[k][2] = ra < nrows ? pa[8 * k + 4 + c] : 0u;
-          qa[k][3] = rb < nrows ? pb[8 * k + 4 + c] : 0u;
-        }
+      for (int k = 0; k < 8; ++k) {
+        qa[k][0] = a ? pa[8 * k + c] : 0u;
+        qa[k][1] = b ? pb[8 * k + c] : 0u;
+        qa[k][2] = a ? pa[8 * k + 4 + c] : 0u;
+        qa[k][3] = b ? pb[8 * k + 4 + c] : 0u;
       }
+    };
+    const NarrowItem* x = items.take();
+    if (x != nullptr) load_q(x);
+    while (x != nullptr) {
+      const int nrows = x->n * G, len = x->len, t0 = x->t0, t1 = x->t1, h = x->h, first_row = x->first;
+      const bool whole = x->whole != 0;
       // positions that the rows see
-      const int la = ra < nrows ? r.len - r.n + ja + 1 : 0, lb = rb < nrows ? r.len - r.n + jb + 1 : 0, all_see = r.len - r.n + 1;
+      const int all_see = len - x->n + 1;
+      const int la = r8 < nrows ? all_see + r8 / G : 0, lb = r8 + 8 < nrows ? all_see + (r8 + 8) / G : 0;
       float ma = -INFINITY, mb = -INFINITY, sa = 0, sb = 0;
       float o[16][4];
 #pragma unroll
-      for (int t = 0; t < 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0;
-      for (int t = t0; t < t1; ++t, step()) {
-        if (int(st & 1u) != side) continue;
-        if (!*abort_flag) mbar_wait_long(&full[st], ph, abort_flag, kPagedTimeoutNs);
-        const uint32_t kt = ring_addr + st * 2 * kNarTileBytes, vt = kt + kNarTileBytes;
-        for (int s16 = 0; s16 < blocks; ++s16) {
-          const int at = slice * 16 * blocks + s16 * 16;  // first position within the tile
+      for (int d = 0; d < 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0;
+      for (int t = t0; t < t1; ++t) {
+        if (int(st & 1u) == side) {
+          items.wait(&full[st], ph);
+          const uint32_t kt = ring_addr + st * 2 * kNarTileBytes, vt = kt + kNarTileBytes;
           const int pos = t * kNarTile + at;
-          if (pos >= r.len) break;
-          float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+          if (pos < len) {
+            float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            uint32_t kf[4];
-            nar_ldmatrix(kf, chunk_addr(kt, at + k_row, 2 * k + k_chunk));
-            mma_16816<T>(s[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[0], kf[1]);
-            mma_16816<T>(s[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[2], kf[3]);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][e] *= args.scale_log2;
-          const bool masked = pos + 16 > all_see;
-          if (masked) {
+            for (int k = 0; k < 8; ++k) {
+              uint32_t kf[4];
+              nar_ldmatrix(kf, chunk_addr(kt, k_row, 2 * k + k_chunk));
+              mma_16816<T>(s[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[0], kf[1]);
+              mma_16816<T>(s[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[2], kf[3]);
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int p = pos + 8 * j + 2 * c + e;
-                if (p >= la) s[j][e] = -INFINITY;
-                if (p >= lb) s[j][2 + e] = -INFINITY;
+              for (int e = 0; e < 4; ++e) s[j][e] *= args.scale_log2;
+            if (pos + 16 > all_see) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int p = pos + 8 * j + 2 * c + e;
+                  if (p >= la) s[j][e] = -INFINITY;
+                  if (p >= lb) s[j][2 + e] = -INFINITY;
+                }
+            }
+            float xa = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), xb = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+              xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, d));
+              xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, d));
+            }
+            if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
+              const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
+              const float ca = na == -INFINITY ? 1.f : exp2_fast(ma - na), cb = nb == -INFINITY ? 1.f : exp2_fast(mb - nb);
+              ma = na;
+              mb = nb;
+              sa *= ca;
+              sb *= cb;
+#pragma unroll
+              for (int d = 0; d < 16; ++d) {
+                o[d][0] *= ca; o[d][1] *= ca; o[d][2] *= cb; o[d][3] *= cb;
               }
-          }
-          float xa = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), xb = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+            }
+            const float ua = ma == -INFINITY ? 0.f : ma, ub = mb == -INFINITY ? 0.f : mb;
+            uint32_t pw[4];  // the weights as the next product's left operand
 #pragma unroll
-          for (int d = 1; d < 4; d <<= 1) {
-            xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, d));
-            xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, d));
-          }
-          if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
-            const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
-            const float ca = na == -INFINITY ? 1.f : exp2_fast(ma - na), cb = nb == -INFINITY ? 1.f : exp2_fast(mb - nb);
-            ma = na;
-            mb = nb;
-            sa *= ca;
-            sb *= cb;
+            for (int j = 0; j < 2; ++j) {
+              const float p0 = exp2_fast(s[j][0] - ua), p1 = exp2_fast(s[j][1] - ua), p2 = exp2_fast(s[j][2] - ub), p3 = exp2_fast(s[j][3] - ub);
+              sa += p0 + p1;
+              sb += p2 + p3;
+              pw[2 * j] = pack2<T>(p0, p1);
+              pw[2 * j + 1] = pack2<T>(p2, p3);
+            }
+            // values of positions that do not exist count as zero (a weight of zero would not do: they may be NaN)
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+            if (pos + 16 > len) {
+              const int left = len - pos - 2 * c;
+              keep0 = left <= 0 ? 0u : left == 1 ? 0xffffu : 0xffffffffu;
+              keep1 = left <= 8 ? 0u : left == 9 ? 0xffffu : 0xffffffffu;
+            }
 #pragma unroll
-            for (int d = 0; d < 16; ++d) {
-              o[d][0] *= ca; o[d][1] *= ca; o[d][2] *= cb; o[d][3] *= cb;
+            for (int d = 0; d < 8; ++d) {
+              uint32_t vf[4];
+              nar_ldmatrix_trans(vf, chunk_addr(vt, v_row, 2 * d + v_chunk));
+              mma_16816<T>(o[2 * d], pw[0], pw[1], pw[2], pw[3], vf[0] & keep0, vf[1] & keep1);
+              mma_16816<T>(o[2 * d + 1], pw[0], pw[1], pw[2], pw[3], vf[2] & keep0, vf[3] & keep1);
             }
           }
-          const float ua = ma == -INFINITY ? 0.f : ma, ub = mb == -INFINITY ? 0.f : mb;
-          uint32_t pw[4];  // the weights as the next product's left operand
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float p0 = exp2_fast(s[j][0] - ua), p1 = exp2_fast(s[j][1] - ua), p2 = exp2_fast(s[j][2] - ub), p3 = exp2_fast(s[j][3] - ub);
-            sa += p0 + p1;
-            sb += p2 + p3;
-            pw[2 * j] = pack2<T>(p0, p1);
-            pw[2 * j + 1] = pack2<T>(p2, p3);
-          }
-          // values of positions that do not exist count as zero (a weight of zero would not do: they may be NaN)
-          uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-          if (pos + 16 > r.len) {
-            const int left = r.len - pos - 2 * c;
-            keep0 = left <= 0 ? 0u : left == 1 ? 0xffffu : 0xffffffffu;
-            keep1 = left <= 8 ? 0u : left == 9 ? 0xffffu : 0xffffffffu;
-          }
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            uint32_t vf[4];
-            nar_ldmatrix_trans(vf, chunk_addr(vt, at + v_row, 2 * d + v_chunk));
-            mma_16816<T>(o[2 * d], pw[0], pw[1], pw[2], pw[3], vf[0] & keep0, vf[1] & keep1);
-            mma_16816<T>(o[2 * d + 1], pw[0], pw[1], pw[2], pw[3], vf[2] & keep0, vf[3] & keep1);
-          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[st]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
+        if (++st == kNarStages) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
+      items.give_back();
+      x = items.take();
+      if (x != nullptr) load_q(x);  // on its way while this item is put together
 #pragma unroll
       for (int d = 1; d < 4; d <<= 1) {
         sa += __shfl_xor_sync(0xffffffffu, sa, d);
         sb += __shfl_xor_sync(0xffffffffu, sb, d);
       }
-      // ---- the odd tiles' warps hand over to the even ones', these to all ---------------------------------------------
-      float* mine = s_o + w4 * 16 * kNarORow;
-      auto put = [&]() {
+      // ---- the warps' parts of rows 0 - 7, then of 8 - 15, are added: a warp per row, four dimensions a lane ------------
+      float* piece = whole ? nullptr : Piece<kNarRows>::slot(args, blockIdx.x, t0 > 0 ? 0 : 1);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) {
-          *reinterpret_cast<float2*>(mine + r8 * kNarORow + 8 * d + 2 * c) = make_float2(o[d][0], o[d][1]);
-          *reinterpret_cast<float2*>(mine + (r8 + 8) * kNarORow + 8 * d + 2 * c) = make_float2(o[d][2], o[d][3]);
-        }
-        if (c == 0) {
-          s_ml[w4][r8] = make_float2(ma, sa);
-          s_ml[w4][r8 + 8] = make_float2(mb, sb);
-        }
-      };
-      if (odd_tiles) {
-        if (side == 1) put();
+      for (int half = 0; half < 2; ++half) {
+        if (half * 8 >= nrows) break;
+        float* mine = s_o + (warp * 8 + r8) * kNarORow;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) *reinterpret_cast<float2*>(mine + 8 * d + 2 * c) = make_float2(o[d][2 * half], o[d][2 * half + 1]);
+        if (c == 0) s_ml[warp][r8] = half == 0 ? make_float2(ma, sa) : make_float2(mb, sb);
         nar_sync();
-        if (side == 0) {
-          const float2 a = s_ml[w4][r8], b = s_ml[w4][r8 + 8];
-          const float na = fmaxf(ma, a.x), nb = fmaxf(mb, b.x);
-          const float ua = na == -INFINITY ? 0.f : na, ub = nb == -INFINITY ? 0.f : nb;
-          const float fa = exp2_fast(ma - ua), fb = exp2_fast(mb - ub), ga = exp2_fast(a.x - ua), gb = exp2_fast(b.x - ub);
-          ma = na;
-          mb = nb;
-          sa = sa * fa + a.y * ga;
-          sb = sb * fb + b.y * gb;
+        const int row = half * 8 + warp;
+        if (row < nrows) {
+          float2 ml[kNarWarps];
+          float m = -INFINITY, l = 0;
 #pragma unroll
-          for (int d = 0; d < 16; ++d) {
-            const float2 x = *reinterpret_cast<const float2*>(mine + r8 * kNarORow + 8 * d + 2 * c);
-            const float2 y = *reinterpret_cast<const float2*>(mine + (r8 + 8) * kNarORow + 8 * d + 2 * c);
-            o[d][0] = o[d][0] * fa + x.x * ga;
-            o[d][1] = o[d][1] * fa + x.y * ga;
-            o[d][2] = o[d][2] * fb + y.x * gb;
-            o[d][3] = o[d][3] * fb + y.y * gb;
+          for (int w = 0; w < kNarWarps; ++w) {
+            ml[w] = s_ml[w][warp];
+            m = fmaxf(m, ml[w].x);
+          }
+          const float u = m == -INFINITY ? 0.f : m;
+          float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+          for (int w = 0; w < kNarWarps; ++w) {
+            const float f = exp2_fast(ml[w].x - u);
+            const float4 y = *reinterpret_cast<const float4*>(s_o + (w * 8 + warp) * kNarORow + lane * 4);
+            l += ml[w].y * f;
+            v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
+          }
+          if (whole) {
+            const float inv = l == 0 ? 0.f : 1 / l;  // a row that sees nothing
+            const int j = row / G;
+            T* dst = static_cast<T*>(args.out) + (int64_t(first_row + j) * args.hq + int64_t(h) * G + (row - j * G)) * kAttnD + lane * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+          } else {
+            if (lane == 0) *reinterpret_cast<float2*>(piece + 2 * row) = make_float2(m, l);
+            *reinterpret_cast<float4*>(piece + 2 * kNarRows + row * kAttnD + lane * 4) = v;
           }
         }
-        __syncwarp();
+        nar_sync();
       }
-      if (side == 0) put();
-      nar_sync();
-      // 32 threads a row, four dimensions each
-      const bool whole = t0 == 0 && t1 == tiles;
-      float* piece = whole ? nullptr : Piece<kNarRows>::slot(args, blockIdx.x, t0 > 0 ? 0 : 1);
-      const int slices = 4 / blocks;
-      for (int row = warp; row < nrows; row += kNarWarps) {
-        const int b = row >> 4, in = row & 15;
-        float m = -INFINITY, l = 0;
-        for (int s = 0; s < slices; ++s) m = fmaxf(m, s_ml[s * blocks + b][in].x);
-        const float u = m == -INFINITY ? 0.f : m;
-        float4 v = make_float4(0, 0, 0, 0);
-        for (int s = 0; s < slices; ++s) {
-          const float2 ml = s_ml[s * blocks + b][in];
-          const float f = exp2_fast(ml.x - u);
-          const float4 x = *reinterpret_cast<const float4*>(s_o + ((s * blocks + b) * 16 + in) * kNarORow + lane * 4);
-          l += ml.y * f;
-          v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
-        }
-        if (whole) {
-          const float inv = l == 0 ? 0.f : 1 / l;  // a row that sees nothing
-          const int j = row / G;
-          T* dst = static_cast<T*>(args.out) + (int64_t(r.row0 + j) * args.hq + int64_t(h) * G + (row - j * G)) * kAttnD + lane * 4;
-          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-        } else {
-          if (lane == 0) *reinterpret_cast<float2*>(piece + 2 * row) = make_float2(m, l);
-          *reinterpret_cast<float4*>(piece + 2 * kNarRows + row * kAttnD + lane * 4) = v;
-        }
-      }
-      nar_sync();
-    });
+    }
   }
+  zero_tail<T>(args);
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) *args.status = 1;
-}
-
-constexpr int kNarJoin = 8;  // warps of a row: one request alone leaves a piece on every SM
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_narrow_join_kernel(const __grid_constant__ PagedArgs args, int spans) {
-  pdl_launch_dependents();
-  pdl_wait();
-  join_rows<T, kNarRows, kNarJoin>(args, spans, [&](const int4& item, int row) -> T* {
-    const Request r = request_at(args, item.x);
-    if (row >= r.n * args.group) return nullptr;
-    const int j = row / args.group;
-    return static_cast<T*>(args.out) + (int64_t(r.row0 + j) * args.hq + int64_t(item.y) * args.group + (row - j * args.group)) * kAttnD;
-  });
 }
 
 }  // namespace b200ipc

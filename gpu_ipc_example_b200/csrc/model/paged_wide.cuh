@@ -1,20 +1,23 @@
-// Attention over a paged cache for requests with many rows: prompts, and chunks of them.
+// Attention over a paged cache for requests with more rows than the narrow kernel's: prompts, chunks of them, drafts of many heads.
 //
 // Rows are (new token, query head) pairs of one KV head, a token's heads next to one another, so that a K or V tile serves all heads of
-// the group.  A CTA takes 256 rows, two accumulator tiles of 128, over tiles of 128 positions:
+// the group.  A CTA takes up to 256 rows over tiles of 128 positions, with two accumulators of 128 rows:
 //
-//   warp 8       streams K and V tiles, page by page, by TMA (128-byte swizzle, no multicast) into a ring of five
-//   warp 10      walks the span and hands its items to the others through a queue in shared memory
-//   warp 9       issues tcgen05.mma: S_w = Q_w K^T into tensor memory, and O_w += P_w V with P_w from tensor memory
-//   warps 0-3, 4-7   softmax of tile w = 0, 1, one row a thread: S out of tensor memory, maximum, weights, sum, P back over S
+//   warp 8       streams K and V tiles, page by page, by TMA (128-byte swizzle, no multicast) into a ring of four
+//   warps 9, 10  issue tcgen05.mma, w = 0 and 1: S_w = Q K^T into tensor memory, and O_w += P_w V with P_w from tensor memory.  One warp
+//                for both spent as long on waits, fences and commits between the products as the tensor cores on these
+//   warps 0-3, 4-7   softmax w = 0, 1, one row a thread: S out of tensor memory, maximum, weights, sum, P back over S
+//   warp 11      walks the span, hands out its items and brings their rows of Q
 //
-// While one tile's softmax runs, the tensor cores work for the other.  Tensor memory is full: 2 x 128 columns S (P over it, 16 bits), 2 x
-// 128 columns O.  The running maximum is only moved when it grows by more than 2^8: till then weights are up to 256 instead of 1, which
-// fp32 sums and 16-bit weights hold alike (relative rounding), and O is left alone (fetching and storing it costs as much as the softmax
-// of a tile).  The order of S_w(j + 1) behind O_w(j) in the one issuing thread is what makes both "P has been read" and "O is complete"
-// follow from "S is there".
+// Items of more than 128 rows: accumulator w is rows 128 w .. of the item, over the same tiles of positions.  Items of up to 128: both have
+// the same rows, w = 0 the even tiles, w = 1 the odd ones, and are added at the end.  Either way the tensor cores work for one of them while
+// the other's softmax runs.  Tensor memory is full: 2 x 128 columns S (P over it, 16 bits), 2 x 128 columns O.  The running maximum is only
+// moved when it grows by more than 2^8: till then weights are up to 256 instead of 1, which fp32 sums and 16-bit weights hold alike
+// (relative rounding), and O is left alone (fetching and storing it costs as much as the softmax of a tile).  The order of S_w(j + 1)
+// behind O_w(j) in the one issuing thread is what makes both "P has been read" and "O is complete" follow from "S is there".
 //
-// Bound by the exponentials: 128 x 128 weights at 16 a clock are 1024 clocks, its two products 1024 on the tensor cores.
+// Bound by the exponentials where rows are many (128 x 128 weights at 16 a clock are 1024 clocks, their two products 1024 on the tensor
+// cores), by memory where they are few.
 #pragma once
 
 #include "paged_work.cuh"
@@ -23,21 +26,32 @@ namespace b200ipc {
 
 constexpr int kWideRows = 256;
 constexpr int kWideTile = 128;   // positions
-constexpr int kWideStages = 5;   // K or V tiles
-constexpr int kWideQueue = 4;    // items handed out ahead
+constexpr int kWideStages = 4;   // K or V tiles
 constexpr int kWideThreads = 384;  // three warpgroups
-constexpr int kWideRegsSoftmax = 224, kWideRegsRest = 56;  // 256 x 208 + 128 x 88 = 384 x 168, what the launch has
+constexpr int kWideRegsSoftmax = 208, kWideRegsRest = 88;  // 256 x 208 + 128 x 88 = 384 x 168, what the launch has
 constexpr int kWideTileBytes = kWideTile * kAttnD * 2;  // also of 128 rows of Q
-constexpr size_t kWideSmem = 1024 + size_t(kWideStages + 2) * kWideTileBytes;
+constexpr int kWideStage = 4096;  // bytes of a softmax warp's way out: 32 rows x 128
+constexpr size_t kWideSmem = 1024 + size_t(kWideStages + 2) * kWideTileBytes + 8 * kWideStage;
 constexpr int kWideStart = 192;  // what an item's start and end cost, in positions
 constexpr int kWideLeast = 384;  // a span is at least so long: more than kWideStart + a tile, so that every cut leaves a tile on both sides
 constexpr float kWideSlack = 8.f;
+
+// The part of an item that lies in a span.
+struct WideItem {
+  int valid;
+  int request, h;       // KV head
+  int first, n, len;    // the request's first row of q, its new tokens, its tokens in the cache
+  int row0, rows;       // rows of the item within the request
+  int t0, t1, whole;    // tiles of positions; whether these are all
+  int split;            // up to 128 rows: the accumulators take tiles in turn
+  int count[2];         // tiles that accumulator w looks at: from t0 on, or every other one
+};
 
 struct WideCut {
   const PagedArgs& a;
   __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0 && r.n * a.group > a.narrow_rows; }
   __device__ __forceinline__ int items(const Request& r) const { return (r.n * a.group + kWideRows - 1) / kWideRows; }
-  // positions that the rows below `row` of the request see
+  // positions that the rows below `rows` of the request see
   __device__ __forceinline__ int seen(const Request& r, int rows) const {
     return rows <= 0 ? 0 : max(0, r.len - r.n + (min(rows, r.n * a.group) - 1) / a.group + 1);
   }
@@ -47,12 +61,15 @@ struct WideCut {
     return t * (int64_t(max(0, r.len - r.n)) + kWideStart) * a.group + (kWideRows / 2) * t * (t + 1);
   }
   __device__ __forceinline__ int64_t length(const Request& r) const { return takes(r) ? a.hkv * before(r, items(r)) : 0; }
-  __device__ __forceinline__ int4 place(const Mark& m) const {
-    if (m.request >= a.requests) return make_int4(a.requests, 0, 0, 0);
+  __device__ __forceinline__ Start start(const Request& r, int request, int h, int item, int n, int tile) const {
+    return Start{request, h * n + item, tile, min(kWideRows, r.n * a.group - item * kWideRows), int64_t(r.row0) * a.hq + int64_t(h) * a.group, item * kWideRows, 0};
+  }
+  __device__ __forceinline__ Start place(const Mark& m) const {
+    if (m.request >= a.requests) return Start{a.requests, 0, 0, 0, 0, 0, 0};
     const Request r = request_at(a, m.request);
     const int n = items(r);
     const int64_t per = before(r, n);
-    const int h = int(m.offset / per);
+    const int h = int(divide(m.offset, per));
     const int64_t rest = m.offset - h * per;
     int lo = 0, hi = n;  // the last item that begins at or before `rest`
     while (hi - lo > 1) {
@@ -61,35 +78,26 @@ struct WideCut {
       else hi = mid;
     }
     const int64_t in = rest - before(r, lo) - int64_t(kWideStart) * a.group;
-    const int t = in <= 0 ? 0 : int((in + int64_t(kWideTile / 2) * a.group) / (int64_t(kWideTile) * a.group));
+    const int t = in <= 0 ? 0 : int(divide(in + int64_t(kWideTile / 2) * a.group, int64_t(kWideTile) * a.group));
     const int all = tiles(r, lo);
     if (t >= all && all > 0) {  // rounded to its end: the next item
-      if (lo + 1 < n) return make_int4(m.request, h * n + lo + 1, 0, 0);
-      if (h + 1 < a.hkv) return make_int4(m.request, (h + 1) * n, 0, 0);
-      return make_int4(m.request + 1, 0, 0, 0);
+      if (lo + 1 < n) return start(r, m.request, h, lo + 1, n, 0);
+      if (h + 1 < a.hkv) return start(r, m.request, h + 1, 0, n, 0);
+      return Start{m.request + 1, 0, 0, 0, 0, 0, 0};
     }
-    return make_int4(m.request, h * n + lo, min(t, max(all - 1, 0)), 0);
+    return start(r, m.request, h, lo, n, min(t, max(all - 1, 0)));
   }
-};
-
-// The part of an item that lies in a span, as the scheduling warp hands it to the others.
-struct WideItem {
-  int valid;
-  int request, h;       // KV head
-  int first, n, len;    // the request's first row of q, its new tokens, its tokens in the cache
-  int row0, rows;       // rows of the item within the request
-  int t0, t1, whole;    // tiles of positions; whether these are all
-  int count[2];         // tiles of positions from t0 on that accumulator tile w looks at
 };
 
 // The span's items one after the other.
 struct WideWalk {
   const PagedArgs& a;
   const WideCut cut;
-  const int4 last;
+  const Start last;
   Window win;
   int i, number, t0;
-  __device__ __forceinline__ WideWalk(const PagedArgs& args, const int4& first, const int4& end) : a(args), cut{args}, last(end), i(first.x), number(first.y), t0(first.z) {}
+  __device__ __forceinline__ WideWalk(const PagedArgs& args, const Start& first, const Start& end)
+      : a(args), cut{args}, last(end), i(first.request), number(first.number), t0(first.tile) {}
   __device__ __forceinline__ WideItem next() {
     WideItem x{};
     const auto takes = [&](const Request& r) { return cut.takes(r); };
@@ -100,7 +108,7 @@ struct WideWalk {
         number = t0 = 0;
       }
     }
-    if (i >= a.requests || i > last.x || (i == last.x && (number > last.y || (number == last.y && t0 >= last.z)))) return x;
+    if (i >= a.requests || i > last.request || (i == last.request && (number > last.number || (number == last.number && t0 >= last.tile)))) return x;
     x.valid = 1;
     const Request r = win.get(i);
     const int n = cut.items(r);
@@ -114,12 +122,17 @@ struct WideWalk {
     x.rows = min(kWideRows, r.n * a.group - x.row0);
     const int tiles = cut.tiles(r, item);
     x.t0 = t0;
-    x.t1 = i == last.x && number == last.y ? last.z : tiles;
+    x.t1 = i == last.request && number == last.number ? last.tile : tiles;
     x.whole = t0 == 0 && x.t1 == tiles;
+    x.split = x.rows <= 128;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const int see = x.rows > w * 128 ? cut.seen(r, x.row0 + min(x.rows, (w + 1) * 128)) : 0;
-      x.count[w] = max(0, min((see + kWideTile - 1) / kWideTile, x.t1) - x.t0);
+      if (x.split) {
+        x.count[w] = (x.t1 - x.t0 + 1 - w) / 2;
+      } else {
+        const int see = cut.seen(r, x.row0 + min(x.rows, (w + 1) * 128));
+        x.count[w] = max(0, min((see + kWideTile - 1) / kWideTile, x.t1) - x.t0);
+      }
     }
     t0 = 0;
     if (++number == a.hkv * n) {
@@ -130,14 +143,11 @@ struct WideWalk {
   }
 };
 
-__device__ __forceinline__ void tmem_st_32cols(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_16cols(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -163,12 +173,51 @@ __device__ __forceinline__ uint64_t make_sw128_nmajor_desc(uint32_t smem_addr) {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// 64 columns x `group` heads x 128 / group tokens of Q: 128 rows of the item
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int half, int h, int token) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(half), "r"(0), "r"(h), "r"(token)
+      : "memory");
+}
+// Two fp32 values in one register pair
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+  return x;
+}
+__device__ __forceinline__ float2 f32x2_parts(uint64_t x) {
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t f32x2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t x;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+  return x;
+}
+__device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
+  uint64_t x;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+  return x;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void wide_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // the softmax warps
+
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __grid_constant__ PagedArgs args) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t kv_full[kWideStages], kv_empty[kWideStages], q_ready[2], s_full[2], p_ready[2], o_full[2], item_full[kWideQueue], item_empty[kWideQueue], mma_done;
-  __shared__ WideItem s_items[kWideQueue];
-  __shared__ Mark s_marks[2];
+  using Items = Queue<WideItem, 11>;  // the softmax warps, the stream, the products
+  __shared__ Items s_queue;
+  __shared__ uint64_t kv_full[kWideStages], kv_empty[kWideStages], q_ready[2], q_free[2], s_full[2], p_ready[2][2], o_full[2], mma_done;
+  __shared__ float2 s_ml[128];  // maxima and sums of w = 1
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   unsigned char* q_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -179,19 +228,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWideStages; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&q_ready[w], 128);
+      mbar_init(&q_ready[w], 1);
+      mbar_init(&q_free[w], 2);
       mbar_init(&s_full[w], 1);
-      mbar_init(&p_ready[w], 128);
+      mbar_init(&p_ready[w][0], 4);  // a warp is one arrival: 128 on one word would stand in line
+      mbar_init(&p_ready[w][1], 4);
       mbar_init(&o_full[w], 1);
     }
-    for (int i = 0; i < kWideQueue; ++i) {
-      mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 10);
-    }
-    mbar_init(&mma_done, 1);
+    mbar_init(&mma_done, 2);
+    s_queue.init();
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -202,92 +250,89 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   __syncwarp();
   tc_fence_before_sync();
   pdl_wait();
+  reset_status(args);
   const WideCut cut{args};
-  find_span<kWideThreads>(args, [&](const Request& r) { return cut.length(r); }, int64_t(kWideLeast) * args.group, s_marks);
+  Mark marks[2];
+  find_span<kWideThreads>(args, [&](const Request& r) { return cut.length(r); }, int64_t(kWideLeast) * args.group, warp == 11, reinterpret_cast<int64_t*>(ring), marks);
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
-  const int4 first = cut.place(s_marks[0]), last = cut.place(s_marks[1]);
-  if (threadIdx.x == 0) {
-    args.starts[blockIdx.x] = first;
-    if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
-  }
-  lead<T>(args);
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!*abort_flag) mbar_wait_long(bar, parity, abort_flag, kPagedTimeoutNs);
-  };
+  QueueEnd<Items, WideItem> items{s_queue, abort_flag};
+  auto wait = [&](uint64_t* bar, uint32_t parity) { items.wait(bar, parity); };
 
-  // The items as a role sees them: one in hand at a time, given back when it is done with.
-  uint32_t item_at = 0, item_ph = 0;
-  auto take = [&]() {  // nullptr behind the last one
-    wait(&item_full[item_at], item_ph);
-    const WideItem* x = &s_items[item_at];
-    return x->valid && !__any_sync(0xffffffffu, *abort_flag) ? x : nullptr;
-  };
-  auto give_back = [&]() {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&item_empty[item_at]);
-    if (++item_at == kWideQueue) {
-      item_at = 0;
-      item_ph ^= 1u;
-    }
-  };
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegsSoftmax));
-    // ---- softmax: thread = row of tile w ------------------------------------------------------------------------------------
+    // ---- softmax: thread = row of the accumulator -----------------------------------------------------------------------
     const int w = warp >> 2, row = (warp & 3) * 32 + lane, G = args.group;
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t s_addr = lane_base + uint32_t(w) * 128u, o_addr = lane_base + 256u + uint32_t(w) * 128u;
-    unsigned char* q_row = q_smem + w * kWideTileBytes + row * 128;
-    uint32_t ph_s = 0, ph_o = 0, ring_at = 0, ring_ph = 0;  // the ring position of the item's first K tile
-    auto load_q = [&](const WideItem* x) {
-      if (x == nullptr || x->rows <= w * 128) return;
-      const int at = x->row0 + w * 128 + row, j = at / G;
-      uint4 v[16];
-      if (w * 128 + row < x->rows) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(args.q) + int64_t(x->first + j) * args.row_stride + (int64_t(x->h) * G + (at - j * G)) * kAttnD);
-#pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = src[c];
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(q_row + (c >> 3) * (kWideTileBytes / 2) + (((c & 7) ^ (row & 7)) << 4)) = v[c];
-      fence_async_smem();
-      mbar_arrive(&q_ready[w]);
-    };
-    const WideItem* x = take();
-    load_q(x);
-    while (x != nullptr) {
-      // fields that are needed after the item has been given back
-      const int n = x->t1 - x->t0, t0 = x->t0, len = x->len, h = x->h, first_row = x->first;
-      const bool whole = x->whole != 0;
-      const WideItem* following;
-      if (x->rows > w * 128) {
-        const int at = x->row0 + w * 128 + row, j = at / G;
-        const bool exists = w * 128 + row < x->rows;
-        const int limit = exists ? len - x->n + j + 1 : 0;  // positions that this row sees
-        const int count = x->count[w], clears = w == 0 ? 0 : x->count[0];  // from which tile on this one uses V first
-        float ref = -INFINITY, sum = 0;  // the maximum that the weights are taken against (log2 domain)
-        for (int t = 0; t < count; ++t) {
-          const int p0 = (t0 + t) * kWideTile;
+    uint32_t ph_s = 0, ph_o = 0, ring_at = 0, ring_ph = 0;  // the ring position of the item's first tile
+    for (const WideItem* x = items.take(); x != nullptr; x = items.take()) {
+      // What is needed once is read or computed again: the loop over the tiles has few registers to spare.
+      const int count = x->count[w], G0 = x->split ? 0 : w * 128;  // first row of this accumulator in the item
+      float ref = -INFINITY, sum = 0;  // the maximum that the weights are taken against (log2 domain)
+      if (G0 < x->rows) {
+        const bool busy = G0 + (warp & 3) * 32 < x->rows;  // this warp has rows
+        // positions that this row sees
+        const int limit = G0 + row < x->rows ? x->len - x->n + (x->row0 + G0 + row) / G + 1 : 0;
+        int p0 = (x->t0 + (x->split ? w : 0)) * kWideTile;
+        for (int t = 0; t < count; ++t, p0 += x->split ? 2 * kWideTile : kWideTile) {
           wait(&s_full[w], ph_s);
           ph_s ^= 1u;
-          tc_fence_after_sync();
-          float s[kWideTile];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32cols(s_addr + uint32_t(c) * 32u, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-          tmem_ld_wait();
-          if (__any_sync(0xffffffffu, limit < p0 + kWideTile)) {
-#pragma unroll
-            for (int c = 0; c < kWideTile; ++c)
-              if (p0 + c >= limit) s[c] = -INFINITY;
+          // Values of positions that do not exist count as zero (a weight of zero would not do: they may be NaN).  They are in the item's last
+          // tile; each softmax that uses it clears them, as neither waits for the other.
+          if (t == count - 1 && x->t1 * kWideTile > x->len) {
+            const int n = x->t1 - x->t0;
+            if (x->split ? ((n - 1) & 1) == w : count == n) {
+              const uint32_t v_at = ring_at + uint32_t(2 * n - 1);  // that tile in the ring
+              const uint32_t v_st = v_at % kWideStages, v_ph = ring_ph ^ ((v_at / kWideStages) & 1u);
+              wait(&kv_full[v_st], v_ph);
+              if (p0 + row >= x->len) {
+                unsigned char* v = ring + v_st * kWideTileBytes + row * 128;
+#pragma unroll 4
+                for (int c = 0; c < 8; ++c) {
+                  *reinterpret_cast<uint4*>(v + (c << 4)) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(v + kWideTileBytes / 2 + (c << 4)) = make_uint4(0, 0, 0, 0);
+                }
+              }
+              fence_async_smem();
+            }
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+          auto half_done = [&](int half) {  // 64 positions' weights are there
+            if (busy) {
+              tmem_st_wait();
+              tc_fence_before_sync();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[w][half]);
+          };
+          if (!busy) {
+            half_done(0);
+            half_done(1);
+            continue;
+          }
+          tc_fence_after_sync();
+          // All 128 columns for the maximum.  The second half of them is fetched once more for the weights, 32 at a time behind the first
+          // half's: 64 registers less.
+          float s[4][32];
+          auto fetch_s = [&](int c) { tmem_ld_32cols(s_addr + uint32_t(c) * 32u, *reinterpret_cast<uint32_t(*)[32]>(&s[c][0])); };
+          const bool masked = __any_sync(0xffffffffu, limit < p0 + kWideTile);
+          auto mask = [&](int c) {
+            if (masked) {
 #pragma unroll
-          for (int c = 4; c < kWideTile; c += 4)
+              for (int e = 0; e < 32; ++e)
+                if (p0 + 32 * c + e >= limit) s[c][e] = -INFINITY;
+            }
+          };
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[c + e]);
+          for (int c = 0; c < 4; ++c) fetch_s(c);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask(c);
+          float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], s[c][e], s[c][e + 1]);
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * args.scale_log2;
           if (__any_sync(0xffffffffu, top > ref + kWideSlack)) {
             const float now = fmaxf(ref, top);
@@ -295,270 +340,362 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
               const float f = now == -INFINITY ? 1.f : exp2_fast(ref - now);
               sum *= f;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint32_t o[32];
-                tmem_ld_32cols(o_addr + uint32_t(c) * 32u, o);
+              for (int c = 0; c < 8; ++c) {
+                uint32_t o[16];
+                tmem_ld_16cols(o_addr + uint32_t(c) * 16u, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st_32cols(o_addr + uint32_t(c) * 32u, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st_16cols(o_addr + uint32_t(c) * 16u, o);
               }
             }
             ref = now;
           }
           const float shift = ref == -INFINITY ? 0.f : -ref;
-          float part[4] = {0, 0, 0, 0};
+          uint64_t part[2] = {0, 0};  // pairs of sums
+          auto weights = [&](int c) {  // 32 positions from 32 c on
+            uint32_t p[16];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float a = exp2_fast(fmaf(s[64 * c + 2 * e], args.scale_log2, shift)), b = exp2_fast(fmaf(s[64 * c + 2 * e + 1], args.scale_log2, shift));
-              part[2 * (e & 1)] += a;
-              part[2 * (e & 1) + 1] += b;
-              p[e] = pack2<T>(a, b);
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t v = f32x2_fma(f32x2(s[c][2 * e], s[c][2 * e + 1]), f32x2(args.scale_log2, args.scale_log2), f32x2(shift, shift));
+              float2 y = f32x2_parts(v);
+              y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+              part[e & 1] = f32x2_add(part[e & 1], f32x2(y.x, y.y));
+              p[e] = pack2<T>(y.x, y.y);
             }
-            tmem_st_32cols(s_addr + uint32_t(c) * 32u, p);
-          }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
-          // Values of positions that do not exist count as zero (a weight of zero would not do: they may be NaN).  Whichever tile uses
-          // this V tile first clears them.
-          if (p0 + kWideTile > len && t >= clears) {
-            const uint32_t v_at = ring_at + uint32_t(2 * t + 1);
-            const uint32_t v_st = v_at % kWideStages, v_ph = ring_ph ^ ((v_at / kWideStages) & 1u);
-            wait(&kv_full[v_st], v_ph);
-            if (p0 + row >= len) {
-              unsigned char* v = ring + v_st * kWideTileBytes + row * 128;
+            tmem_st_16cols(s_addr + uint32_t(c) * 16u, p);  // over columns that are not needed any more
+          };
+          weights(0);
+          fetch_s(2);
+          weights(1);
+          half_done(0);
+          tmem_ld_wait();
+          fetch_s(3);
+          mask(2);
+          weights(2);
+          tmem_ld_wait();
+          mask(3);
+          weights(3);
+          half_done(1);
+          const float2 a = f32x2_parts(f32x2_add(part[0], part[1]));
+          sum += a.x + a.y;
+        }
+      }
+      // ---- the end of the item ---------------------------------------------------------------------------------------------------
+      const bool split = x->split != 0, whole = x->whole != 0, both = split && x->t1 - x->t0 > 1;
+      const bool busy = G0 + (warp & 3) * 32 < x->rows, exists = G0 + row < x->rows;
+      const int at = x->row0 + G0 + row, j = at / G;
+      // a row that sees nothing of this accumulator's positions (it sees the first so many)
+      if (!exists || x->len - x->n + j + 1 <= (x->t0 + (split ? w : 0)) * kWideTile) {
+        ref = -INFINITY;
+        sum = 0;
+      }
+      if (count > 0) {
+        wait(&o_full[w], ph_o);
+        ph_o ^= 1u;
+        tc_fence_after_sync();
+      }
+      // Rows leave by 128 bytes: through 4 KB of the warp's own, 16-byte chunks swapped by row, eight lanes a row.  (A row a lane, as the
+      // accumulator comes, is 32 lines for every store, and cost 8 us an item.)
+      unsigned char* way = ring + kWideStages * kWideTileBytes + warp * kWideStage;
+      char* const mine = whole ? reinterpret_cast<char*>(static_cast<T*>(args.out) + (int64_t(x->first + j) * args.hq + int64_t(x->h) * G + (at - j * G)) * kAttnD)
+                               : reinterpret_cast<char*>(Piece<kWideRows>::slot(args, int(blockIdx.x), x->t0 > 0 ? 0 : 1) + 2 * kWideRows + size_t(G0 + row) * kAttnD);
+      const int first_row = G0 + (warp & 3) * 32, rows = x->rows;
+      auto leave = [&](int bytes) {  // what is in the warp's memory goes to `bytes` behind each row's start
+        __syncwarp();
 #pragma unroll
-              for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(v + (c >> 3) * (kWideTileBytes / 2) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_smem();
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3);
+          char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
+          const uint4 v = *reinterpret_cast<const uint4*>(way + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          if (first_row + r < rows) *reinterpret_cast<uint4*>(to + bytes + (lane & 7) * 16) = v;
+        }
+        __syncwarp();
+      };
+      auto chunk = [&](int c) { return reinterpret_cast<uint4*>(way + lane * 128 + ((c ^ (lane & 7)) << 4)); };
+      auto put = [&](const uint32_t (&o)[32], int c) {  // dimensions c .. c + 31
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            auto two = [&](int k) { return pack2<T>(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1])); };
+            *chunk(((c & 32) + e) >> 3) = make_uint4(two(0), two(1), two(2), two(3));
           }
-          tmem_st_wait();
+          if (c & 32) leave((c & 64) * 2);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *chunk(e >> 2) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          leave(c * 4);
+        }
+      };
+      // Where both accumulators have the same rows, w = 0 adds them: every warp can read its 32 rows of all of tensor memory.
+      float f = 1, g = 0;
+      if (both) {
+        if (w == 1) {
+          s_ml[row] = make_float2(ref, sum);
           tc_fence_before_sync();
-          mbar_arrive(&p_ready[w]);
         }
-        give_back();
-        following = take();
-        load_q(following);  // S of this item is complete, so Q is free
-        if (count > 0) {
-          wait(&o_full[w], ph_o);
-          ph_o ^= 1u;
-          tc_fence_after_sync();
-        }
+        wide_sync();
+        tc_fence_after_sync();
+        const float2 other = s_ml[row];
+        const float m = fmaxf(ref, other.x), u = m == -INFINITY ? 0.f : m;
+        f = exp2_fast(ref - u);
+        g = exp2_fast(other.x - u);
+        sum = sum * f + other.y * g;
+        ref = m;
+      }
+      if ((!split || w == 0) && busy) {
+        if (exists && !whole) *reinterpret_cast<float2*>(Piece<kWideRows>::slot(args, int(blockIdx.x), x->t0 > 0 ? 0 : 1) + 2 * (G0 + row)) = make_float2(ref, sum);
         if (whole) {
           const float inv = sum == 0 ? 0.f : 1 / sum;  // a row that sees nothing
-          T* dst = static_cast<T*>(args.out) + (int64_t(first_row + j) * args.hq + int64_t(h) * G + (at - j * G)) * kAttnD;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            if (count > 0) {
-              tmem_ld_32cols(o_addr + uint32_t(c) * 32u, o);
-              tmem_ld_wait();
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(sum == 0 ? 0.f : __uint_as_float(o[e]) * inv);
-            if (exists) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                auto pair = [&](int k) { return pack2<T>(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1])); };
-                *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(pair(0), pair(1), pair(2), pair(3));
-              }
-            }
-          }
-        } else {
-          float* piece = Piece<kWideRows>::slot(args, int(blockIdx.x), t0 > 0 ? 0 : 1);
-          const int r = w * 128 + row;
-          if (exists) *reinterpret_cast<float2*>(piece + 2 * r) = make_float2(ref, sum);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            if (count > 0) {
-              tmem_ld_32cols(o_addr + uint32_t(c) * 32u, o);
-              tmem_ld_wait();
-            }
-            if (exists) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const bool some = count > 0;
-                *reinterpret_cast<uint4*>(piece + 2 * kWideRows + size_t(r) * kAttnD + 32 * c + e) =
-                    some ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0, 0, 0, 0);
-              }
-            }
-          }
+          f *= inv;
+          g *= inv;
         }
-        tc_fence_before_sync();  // O may be written again once this thread's next weights are there
-      } else {
-        give_back();
-        following = take();
-        load_q(following);
+#pragma unroll 1
+        for (int c = 0; c < kAttnD; c += 32) {
+          uint32_t o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+          if (count > 0) {
+            tmem_ld_32cols(o_addr + uint32_t(c), o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = f != 0 && sum != 0 ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+          }
+          if (both) {
+            uint32_t y[32];
+            tmem_ld_32cols(o_addr + 128u + uint32_t(c), y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + (g != 0 && sum != 0 ? __uint_as_float(y[e]) * g : 0.f));
+          }
+          put(o, c);
+        }
       }
-      const uint32_t moved = ring_at + uint32_t(2 * n);
+      tc_fence_before_sync();  // O may be written again once this thread's next weights are there
+      if (both) wide_sync();   // of w = 1 as well
+      const uint32_t moved = ring_at + uint32_t(2 * (x->t1 - x->t0));
       ring_ph ^= (moved / kWideStages) & 1u;
       ring_at = moved % kWideStages;
-      x = following;
+      items.give_back();
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsRest));
     if (warp == 8) {
-      // ---- the stream: lane l loads box l / 2 of a tile, left or right half of the dimensions --------------------------------
+      // ---- the stream: K(0), then K(j + 1) and V(j) in turn.  Lane l knows where box l of a tile is. ------------------------
       const int box = min(args.page, 64), boxes = kWideTile / box, per_page = args.page / box;
-      const int sub = lane >> 1, half = lane & 1;
-      const int64_t outside = args.pages * args.hkv * args.page;
+      const int outside = int(args.pages * args.hkv * args.page);
       uint32_t st = 0, ph = 0;
       int issued = 0;
-      for (const WideItem* x = take(); x != nullptr; x = take()) {
-        const int* table = args.table + int64_t(x->request) * args.width;
-        const int len = x->len, h = x->h, pages = (len + args.page - 1) / args.page, t1 = x->t1;
-        int base = -64, entry = 0;
-        for (int t = x->t0; t < t1; ++t) {
-          const int b = t * boxes + sub, p = b / per_page, offset = (b - p * per_page) * box;
-          const int p_first = t * boxes / per_page;
-          if (p_first < base || (t * boxes + boxes - 1) / per_page >= base + 32) {
-            base = p_first;
-            entry = base + lane < pages ? table[base + lane] : -1;
+      auto load = [&](const CUtensorMap* map, int at, int n) {
+        wait(&kv_empty[st], ph ^ 1u);
+        if (__any_sync(0xffffffffu, *abort_flag)) return;
+        if (lane == 0) mbar_expect_tx(&kv_full[st], uint32_t(n * box) * kAttnD * 2u);
+        __syncwarp();
+        unsigned char* dst = ring + st * kWideTileBytes;
+        for (int k = 0; k < n; ++k, dst += box * 128) {
+          const int row = __shfl_sync(0xffffffffu, at, k);
+          if (elect_one()) {
+            tma_load_2d(dst, map, &kv_full[st], 0, row);
+            tma_load_2d(dst + kWideTileBytes / 2, map, &kv_full[st], 64, row);
           }
-          const int64_t id = __shfl_sync(0xffffffffu, entry, min(31, p - base));
-          const int n = min(boxes, (len - t * kWideTile + box - 1) / box);  // boxes that hold positions of the request
-          const int row = int(id >= 0 && id < args.pages ? (id * args.hkv + h) * args.page + offset : outside);
-  #pragma unroll
-          for (int value = 0; value < 2; ++value) {
-            wait(&kv_empty[st], ph ^ 1u);
-            if (!__any_sync(0xffffffffu, *abort_flag)) {
-              if (lane == 0) mbar_expect_tx(&kv_full[st], uint32_t(n * box) * kAttnD * 2u);
-              __syncwarp();
-              if (sub < n) tma_load_2d(ring + st * kWideTileBytes + half * (kWideTileBytes / 2) + sub * box * 128, value ? &args.tma_v : &args.tma_k, &kv_full[st], half * 64, row);
-              ++issued;
-              if (++st == kWideStages) {
-                st = 0;
-                ph ^= 1u;
-              }
-            }
-          }
+          __syncwarp();
         }
-        give_back();
+        ++issued;
+        if (++st == kWideStages) {
+          st = 0;
+          ph ^= 1u;
+        }
+      };
+      for (const WideItem* x = items.take(); x != nullptr; x = items.take()) {
+        const int* table = args.table + int64_t(x->request) * args.width;
+        const int len = x->len, h = x->h, t0 = x->t0, t1 = x->t1, pages = (len + args.page - 1) / args.page;
+        int base = -64, entry = 0, at = 0, n = 0;  // the tile whose V comes next
+        for (int t = t0; t <= t1 && t1 > t0; ++t) {
+          int k_at = 0, k_n = 0;
+          if (t < t1) {
+            const int b = t * boxes + (lane & (boxes - 1)), p = b / per_page;
+            if ((t * boxes + boxes - 1) / per_page >= base + 32) {
+              base = t * boxes / per_page;
+              entry = base + lane < pages ? table[base + lane] : -1;
+            }
+            const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
+            k_at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
+            k_n = min(boxes, (len - t * kWideTile + box - 1) / box);  // boxes that hold positions of the request
+            load(&args.tma_k, k_at, k_n);
+          }
+          if (t > t0) load(&args.tma_v, at, n);
+          at = k_at;
+          n = k_n;
+        }
+        items.give_back();
       }
       const uint64_t since = globaltimer_ns();
       for (int back = 1; back <= min(issued, kWideStages); ++back)
         mbar_drain(&kv_full[(issued - back) % kWideStages], uint32_t((issued - back) / kWideStages) & 1u, since);
-    } else if (warp == 9) {
-      // ---- the products ----------------------------------------------------------------------------------------------------
-      const uint32_t idesc_s = make_idesc<T>(128, kWideTile), idesc_o = make_idesc<T>(128, kAttnD) | (1u << 16);
-      const uint32_t q_addr = smem_u32(q_smem), ring_addr = smem_u32(ring);
-      uint32_t ring_at = 0, ring_ph = 0;  // the next tile that has not been waited for
-      uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
-      auto next_tile = [&]() {
-        wait(&kv_full[ring_at], ring_ph);
-        const uint32_t st = ring_at;
-        if (++ring_at == kWideStages) {
-          ring_at = 0;
-          ring_ph ^= 1u;
-        }
-        return st;
-      };
-      // 64 columns of a K-major tile are one block of it, 16 of them 32 bytes of its rows; descriptors count in 16 bytes
-      const uint64_t q_desc = make_sw128_kmajor_desc(q_addr), k_desc = make_sw128_kmajor_desc(ring_addr), v_desc = make_sw128_nmajor_desc(ring_addr);
-      constexpr uint64_t kTileStep = kWideTileBytes >> 4, kBlockStep = kWideTileBytes >> 5;
-      auto scores = [&](int w, uint32_t k_st) {
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint64_t a = q_desc + uint64_t(w) * kTileStep, b = k_desc + uint64_t(k_st) * kTileStep;
-  #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t at = uint64_t(k >> 2) * kBlockStep + uint64_t(k & 3) * 2u;
-            umma_f16(tmem + uint32_t(w) * 128u, a + at, b + at, idesc_s, k > 0 ? 1u : 0u);
+    } else if (warp < 11) {
+      // ---- the products of accumulator w: one thread ---------------------------------------------------------------------------
+      if (elect_one()) {
+        const int w = warp - 9;
+        const uint32_t idesc_s = make_idesc<T>(128, kWideTile), idesc_o = make_idesc<T>(128, kAttnD) | (1u << 16);
+        const uint32_t t_s = tmem + uint32_t(w) * 128u, t_o = t_s + 256u;
+        // 64 columns of a K-major tile are one block of it, 16 of them 32 bytes of its rows; descriptors count in 16 bytes
+        const uint64_t q_desc = make_sw128_kmajor_desc(smem_u32(q_smem)), k_desc = make_sw128_kmajor_desc(smem_u32(ring)), v_desc = make_sw128_nmajor_desc(smem_u32(ring));
+        constexpr uint64_t kTileStep = kWideTileBytes >> 4, kBlockStep = kWideTileBytes >> 5;
+        struct Place {
+          uint32_t st, ph;
+        };
+        Place at{0, 0};  // the ring's next tile
+        auto next = [&]() {
+          const Place p = at;
+          if (++at.st == kWideStages) at = Place{0, at.ph ^ 1u};
+          return p;
+        };
+        uint32_t ph_q0 = 0, ph_q1 = 0, ph_p = 0;
+        // Both threads wait for every tile, in order, and both have to give it back, also where only one uses it: copies land out of order, and
+        // a wait for a stage's next round must come from who has seen the round before, and find the round it waits for still there.  The
+        // same with Q.
+        auto landed = [&](const Place& p) { wait(&kv_full[p.st], p.ph); };
+        auto scores = [&](uint64_t q, const Place& p) {
+          tc_fence_after_sync();
+          const uint64_t k = k_desc + uint64_t(p.st) * kTileStep;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint64_t o = uint64_t(i >> 2) * kBlockStep + uint64_t(i & 3) * 2u;
+            umma_f16(t_s, q + o, k + o, idesc_s, i > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[w]);
-        }
-        __syncwarp();
-      };
-      auto outputs = [&](int w, uint32_t v_st, bool fresh) {
-        wait(&p_ready[w], ph_p[w]);
-        ph_p[w] ^= 1u;
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint64_t b = v_desc + uint64_t(v_st) * kTileStep;
-  #pragma unroll
-          for (int k = 0; k < kWideTile / 16; ++k)  // 16 positions: 8 columns of P, 2048 bytes of V
-            umma_f16_ts(tmem + 256u + uint32_t(w) * 128u, tmem + uint32_t(w) * 128u + uint32_t(k) * 8u, b + uint64_t(k) * 128u, idesc_o, !fresh || k > 0 ? 1u : 0u);
-        }
-        __syncwarp();
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) umma_commit(bar);
-        __syncwarp();
-      };
-      for (const WideItem* x = take(); x != nullptr; x = take()) {
-        const int n = x->t1 - x->t0, count[2] = {x->count[0], x->count[1]};
-  #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (x->rows > w * 128) {
-            wait(&q_ready[w], ph_q[w]);
-            ph_q[w] ^= 1u;
+        };
+        auto outputs = [&](bool fresh, const Place& p) {  // in two halves, as P comes
+          const uint64_t v = v_desc + uint64_t(p.st) * kTileStep;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            wait(&p_ready[w][half], ph_p);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < kWideTile / 32; ++i) {  // 16 positions: 8 columns of P, 2048 bytes of V
+              const int k = half * (kWideTile / 32) + i;
+              umma_f16_ts(t_o, t_s + uint32_t(k * 8), v + uint64_t(k) * 128u, idesc_o, !fresh || k > 0 ? 1u : 0u);
+            }
           }
-        }
-        if (n > 0) {
-          const uint32_t st = next_tile();
-  #pragma unroll
-          for (int w = 0; w < 2; ++w)
-            if (count[w] > 0) scores(w, st);
-          commit(&kv_empty[st]);
-        }
-        for (int j = 0; j < n; ++j) {
-          const uint32_t v_st = next_tile(), k_st = j + 1 < n ? next_tile() : 0u;
-  #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (j < count[w]) outputs(w, v_st, j == 0);
-            if (w == 0 ? count[1] <= j : j < count[1]) commit(&kv_empty[v_st]);  // its last reader
-            if (j + 1 < count[w]) scores(w, k_st);
-            else if (j + 1 == count[w]) commit(&o_full[w]);
+          ph_p ^= 1u;
+        };
+        for (const WideItem* x = items.take_alone(); x != nullptr; x = items.take_alone()) {
+          const int n = x->t1 - x->t0, count = x->count[w];
+          const bool split = x->split != 0;
+          wait(&q_ready[0], ph_q0);
+          ph_q0 ^= 1u;
+          if (!split) {
+            wait(&q_ready[1], ph_q1);
+            ph_q1 ^= 1u;
           }
-          if (j + 1 < n) commit(&kv_empty[k_st]);
+          mbar_arrive(&q_free[split ? 1 : 1 - w]);  // what is not used or the other's
+          const uint64_t q = q_desc + uint64_t(split ? 0 : w) * kTileStep;
+          uint64_t* q_done = &q_free[split ? 0 : w];
+          int scored = 0, done = 0;  // tiles whose S, whose O has been issued
+          auto score = [&](const Place& p) {
+            scores(q, p);
+            if (++scored == count) umma_commit(q_done);
+          };
+          auto output = [&](const Place& p) {
+            outputs(done == 0, p);
+            if (++done == count) umma_commit(&o_full[w]);
+          };
+          if (count == 0) mbar_arrive(q_done);
+          // The ring has K(0), then K(j + 1) and V(j) in turn.  `mine`: this accumulator looks at tile j.
+          auto mine = [&](int j) { return split ? (j & 1) == w : j < count; };
+          auto release = [&](const Place& p, bool used) {
+            if (used) umma_commit(&kv_empty[p.st]);
+            else mbar_arrive(&kv_empty[p.st]);
+          };
+          if (n > 0) {
+            const Place k = next();
+            landed(k);
+            if (mine(0)) score(k);
+            release(k, mine(0));
+          }
+          for (int j = 0; j < n; ++j) {
+            const bool more = j + 1 < n;
+            const Place k = more ? next() : at, v = next();
+            if (more) landed(k);
+            if (split) {  // K(j + 1) and V(j) are not the same one's
+              if (more) {
+                if (mine(j + 1)) score(k);
+                release(k, mine(j + 1));
+              }
+              landed(v);
+              if (mine(j)) output(v);
+              release(v, mine(j));
+            } else {  // P(j) has to be read before S(j + 1) goes over it
+              landed(v);
+              if (mine(j)) output(v);
+              release(v, mine(j));
+              if (more) {
+                if (mine(j + 1)) score(k);
+                release(k, mine(j + 1));
+              }
+            }
+          }
+          items.give_back_alone();
         }
-        give_back();
+        umma_commit(&mma_done);
+        mbar_drain(&mma_done, 0, globaltimer_ns());
       }
-      commit(&mma_done);
-      mbar_drain(&mma_done, 0, globaltimer_ns());
-    } else if (warp == 10) {
-      // ---- the items -----------------------------------------------------------------------------------------------------------
-      WideWalk walk(args, first, last);
-      for (bool more = true; more;) {
+      __syncwarp();
+    } else {
+      // ---- the walk, and Q: by TMA where a tile of 128 rows is whole tokens, else 16 lanes a row, one 16-byte chunk each -----------
+      const Start first_item = cut.place(marks[0]), last = cut.place(marks[1]);
+      if (lane == 0) {
+        args.starts[blockIdx.x] = first_item;
+        if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
+      }
+      WideWalk walk(args, first_item, last);
+      uint32_t ph = 1;
+      int sent[2] = {0, 0};
+      for (;;) {
         const WideItem x = walk.next();
-        wait(&item_empty[item_at], item_ph ^ 1u);
-        more = x.valid && !__any_sync(0xffffffffu, *abort_flag);
-        if (lane == 0) {
-          s_items[item_at] = x;
-          mbar_arrive(&item_full[item_at]);
+        if (!items.put(x)) break;
+        const int G = args.group;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          wait(&q_free[w], ph);
+          if (w * 128 >= x.rows || __any_sync(0xffffffffu, *abort_flag)) continue;
+          if (args.q_boxes) {
+            if (elect_one()) {
+              mbar_expect_tx(&q_ready[w], kWideTileBytes);
+              for (int half = 0; half < 2; ++half)
+                tma_load_5d(q_smem + w * kWideTileBytes + half * (kWideTileBytes / 2), &args.tma_q, &q_ready[w], half, x.h, x.first + (x.row0 + w * 128) / G);
+            }
+            __syncwarp();
+            ++sent[w];
+          } else {
+            const int c = lane & 15;
+            const uint32_t to = smem_u32(q_smem) + uint32_t(w) * kWideTileBytes + uint32_t(c >> 3) * (kWideTileBytes / 2);
+            const T* base = static_cast<const T*>(args.q) + int64_t(x.first) * args.row_stride + int64_t(x.h) * G * kAttnD + c * 8;
+            for (int r = w * 128 + (lane >> 4); r < min(x.rows, (w + 1) * 128); r += 2) {
+              const int j = (x.row0 + r) / G, in = r & 127;
+              cp_async_16(to + uint32_t(in) * 128u + uint32_t(((c & 7) ^ (in & 7)) << 4), base + int64_t(j) * args.row_stride + (x.row0 + r - j * G) * kAttnD);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready[w]);
+          }
         }
-        __syncwarp();
-        if (++item_at == kWideQueue) {
-          item_at = 0;
-          item_ph ^= 1u;
-        }
+        ph ^= 1u;
       }
+      const uint64_t since = globaltimer_ns();
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (sent[w] > 0) mbar_drain(&q_ready[w], uint32_t(sent[w] - 1) & 1u, since);
     }
   }
   __syncwarp();
+  zero_tail<T>(args);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   if (warp == 9) tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag) *args.status = 1;
-}
-
-constexpr int kWideJoin = 4;  // warps of a row
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_wide_join_kernel(const __grid_constant__ PagedArgs args, int spans) {
-  pdl_launch_dependents();
-  pdl_wait();
-  join_rows<T, kWideRows, kWideJoin>(args, spans, [&](const int4& mark, int row) -> T* {
-    const WideCut cut{args};
-    const Request r = request_at(args, mark.x);
-    const int n = cut.items(r), h = mark.y / n, at = (mark.y - h * n) * kWideRows + row;
-    if (at >= r.n * args.group) return nullptr;
-    const int j = at / args.group;
-    return static_cast<T*>(args.out) + (int64_t(r.row0 + j) * args.hq + int64_t(h) * args.group + (at - j * args.group)) * kAttnD;
-  });
 }
 
 }  // namespace b200ipc

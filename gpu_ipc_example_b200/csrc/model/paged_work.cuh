@@ -4,11 +4,11 @@
 // the positions they see, in tiles of positions.  All items follow one another on one axis, each as long as its tiles and a constant for
 // its start and end; the axis is cut into equal spans, one per CTA (one per SM).  So nobody waits for a longest request, and a single long
 // one uses the whole GPU.  Every CTA finds its span itself from the lengths on the GPU: one round of loads and a scan, and the same
-// rounding everywhere.
+// rounding everywhere.  One warp of it then walks the span and hands the items to the others through a queue in shared memory.
 //
-// An item that a cut goes through leaves pieces: fp32 sums, maxima and unscaled outputs in the workspace.  A CTA has at most two, the end of an
-// item that began in an earlier span (slot 0) and the beginning of one that goes on in the next (slot 1); the join walks them in order, so the result does not
-// depend on timing.
+// An item that a cut goes through leaves pieces: fp32 sums, maxima and unscaled outputs in the workspace.  A CTA has at most two, the end
+// of an item that began in an earlier span (slot 0) and the beginning of one that goes on in the next (slot 1); the join walks them in
+// order, so the result does not depend on timing.
 #pragma once
 
 #include "../common/check.h"
@@ -19,20 +19,32 @@
 namespace b200ipc {
 
 constexpr uint64_t kPagedTimeoutNs = 2000000000;  // a wait inside a CTA takes microseconds
+constexpr int kPagedQueue = 4;                    // items handed out ahead
+
+// Where a span starts: on tile `tile` of an item, and what the join has to know of that item.
+struct Start {
+  int request, number, tile;  // number: of the request's items, KV head by KV head
+  int rows;                   // of the item
+  int64_t out_row0;           // (first row of q) x hq + first head: a request's row r is out row out_row0 + r / group x hq + r % group
+  int row0, pad;              // its first row within the request
+};
+static_assert(sizeof(Start) == 32);
 
 struct PagedArgs {
   alignas(64) CUtensorMap tma_k, tma_v;  // [pages * hkv * page, 128], boxes of 64 columns x min(page, 64) rows
+  alignas(64) CUtensorMap tma_q;         // [rows, hkv, group, 2, 64], boxes of 128 (row, head) pairs x 64 columns; wide kernel only
   const void* q;
   void* out;
   const int *table, *lens, *cu_new;
-  int4* starts;     // [CTAs + 1]: request, item of it, tile: where each span starts
-  float* part;      // [CTAs][2][piece rows][2 + 128]: see Piece
+  Start* starts;    // [CTAs + 1]
+  float* part;      // [CTAs][2] pieces
   int* status;      // 0, or 1 when a wait gave up
   int64_t row_stride;
   int rows, requests, hq, hkv, group;
   int page, width;
   int64_t pages;
   int narrow_rows;  // items of up to so many rows belong to the narrow kernel, the others to the wide one
+  int q_boxes;      // whether tma_q is there: 128 is a multiple of the group
   int leads;        // the call's first kernel: resets the status, and writes the rows behind the last request
   float scale_log2;
 };
@@ -49,9 +61,10 @@ struct Request {
 };
 __device__ __forceinline__ Request request_at(const PagedArgs& a, int i) {
   Request r;
-  r.row0 = min(max(a.cu_new[i], 0), a.rows);
-  r.n = min(max(a.cu_new[i + 1], r.row0), a.rows) - r.row0;
-  r.len = min(max(a.lens[i], 0), a.width * a.page);
+  const int from = a.cu_new[i], to = a.cu_new[i + 1], len = a.lens[i];
+  r.row0 = min(max(from, 0), a.rows);
+  r.n = min(max(to, r.row0), a.rows) - r.row0;
+  r.len = min(max(len, 0), a.width * a.page);
   return r;
 }
 
@@ -84,49 +97,132 @@ struct Mark {
   int request;
   int64_t offset;  // on the request's own part of the axis
 };
-// Start and end of this CTA's span; for all threads of the block (THREADS of them).  `length` of a request: its part of the axis, 0 for one
-// that is not this kernel's.  No span is shorter than `least` but where the axis ends.
+// Start and end of this CTA's span.  All threads of the block take part, the marks are the walking warp's (`walks`).  `length` of a request:
+// its part of the axis, 0 for one that is not this kernel's.  No span is shorter than `least` but where the axis ends.  s_sum: THREADS words of
+// the ring, which nothing is copied to yet.
+// Divisions of 64-bit integers cost 300 clocks each here, ten of them 1.5 us of a call of ten; so quotients are fp64 products, which round
+// alike in all CTAs and grow with the span's number: all that the cuts need.
 template <int THREADS, typename Length>
-__device__ __forceinline__ void find_span(const PagedArgs& a, Length length, int64_t least, Mark* s_marks /* shared [2] */) {
-  __shared__ int64_t s_sum[THREADS / 32];
-  const int lane = int(threadIdx.x & 31), warp = int(threadIdx.x >> 5);
-  const int each = (a.requests + THREADS - 1) / THREADS, i0 = min(a.requests, int(threadIdx.x) * each), i1 = min(a.requests, i0 + each);
+__device__ __forceinline__ void find_span(const PagedArgs& a, Length length, int64_t least, bool walks, int64_t* s_sum, Mark (&marks)[2]) {
+  __shared__ Mark s_marks[2];
+  constexpr int kPer = THREADS / 32;
+  const int each = (a.requests + THREADS - 1) / THREADS;
+  const int i0 = min(a.requests, int(threadIdx.x) * each), i1 = min(a.requests, i0 + each);
   int64_t mine = 0;
   for (int i = i0; i < i1; ++i) mine += length(request_at(a, i));
-  int64_t in = mine;
+  s_sum[threadIdx.x] = mine;
+  __syncthreads();
+  if (!walks) return;
+  const int lane = int(threadIdx.x & 31);
+  if (lane < 2) s_marks[lane] = {a.requests, 0};
+  int64_t v[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) sum += v[j] = s_sum[lane * kPer + j];
+  int64_t in = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t x = __shfl_up_sync(0xffffffffu, in, o);
     if (lane >= o) in += x;
   }
-  if (lane == 31) s_sum[warp] = in;
-  if (threadIdx.x < 2) s_marks[threadIdx.x] = {a.requests, 0};
-  __syncthreads();
-  int64_t before = in - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
-  const int64_t spans = min(int64_t(gridDim.x), max(int64_t(1), total / least));
+  const int64_t total = __shfl_sync(0xffffffffu, in, 31);
+  const double spans = fmin(double(gridDim.x), fmax(1.0, floor(double(total) * (1.0 / double(least)))));
+  const double per_span = double(total) / spans;
+  __syncwarp();
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int64_t c = int64_t(blockIdx.x) + k;
-    const int64_t at = c >= spans ? total : total / spans * c + total % spans * c / spans;
-    if (at >= before && at < before + mine) {
-      int64_t o = at - before;
-      for (int i = i0; i < i1; ++i) {
-        const int64_t len = length(request_at(a, i));
-        if (o < len) {
-          s_marks[k] = {i, o};
-          break;
+    const int c = int(blockIdx.x) + k;
+    const int64_t at = double(c) >= spans ? total : min(total, int64_t(per_span * double(c)));
+    int64_t before = in - sum;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (at >= before && at < before + v[j]) {
+        int64_t o = at - before;
+        const int t = lane * kPer + j;
+        for (int i = t * each; i < min(a.requests, (t + 1) * each); ++i) {
+          const int64_t len = each == 1 ? v[j] : length(request_at(a, i));
+          if (o < len) {
+            s_marks[k] = {i, o};
+            break;
+          }
+          o -= len;
         }
-        o -= len;
       }
+      before += v[j];
     }
   }
-  __syncthreads();
+  __syncwarp();
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies may go there now
+  marks[0] = s_marks[0];
+  marks[1] = s_marks[1];
 }
+// floor(x / y) of whole numbers below 2^53, by a product with the quotient put right
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  int64_t q = int64_t(double(x) / double(y));
+  if (q * y > x) --q;
+  else if (x - q * y >= y) ++q;
+  return q;
+}
+
+// The queue: the walking warp fills a place, READERS warps give it back.
+template <typename Item, int READERS>
+struct Queue {
+  uint64_t full[kPagedQueue], empty[kPagedQueue];
+  Item items[kPagedQueue];
+  __device__ void init() {
+    for (int i = 0; i < kPagedQueue; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], READERS);
+    }
+  }
+};
+// One warp's place in it.
+template <typename Q, typename Item>
+struct QueueEnd {
+  Q& q;
+  volatile int* abort_flag;
+  uint32_t at = 0, ph = 0;
+  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
+    if (!mbar_try_wait(bar, parity) && !*abort_flag) mbar_wait_long(bar, parity, abort_flag, kPagedTimeoutNs);
+  }
+  __device__ __forceinline__ void step() {
+    if (++at == kPagedQueue) {
+      at = 0;
+      ph ^= 1u;
+    }
+  }
+  // nullptr behind the last item
+  __device__ __forceinline__ const Item* take() {
+    wait(&q.full[at], ph);
+    const Item* x = &q.items[at];
+    return x->valid && !__any_sync(0xffffffffu, *abort_flag) ? x : nullptr;
+  }
+  __device__ __forceinline__ void give_back() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&q.empty[at]);
+    step();
+  }
+  // The same for one thread by itself
+  __device__ __forceinline__ const Item* take_alone() {
+    wait(&q.full[at], ph);
+    const Item* x = &q.items[at];
+    return x->valid && !*abort_flag ? x : nullptr;
+  }
+  __device__ __forceinline__ void give_back_alone() {
+    mbar_arrive(&q.empty[at]);
+    step();
+  }
+  // false when nothing more is wanted
+  __device__ __forceinline__ bool put(const Item& x) {
+    wait(&q.empty[at], ph ^ 1u);
+    if ((threadIdx.x & 31) == 0) {
+      q.items[at] = x;
+      mbar_arrive(&q.full[at]);
+    }
+    __syncwarp();
+    step();
+    return x.valid && !__any_sync(0xffffffffu, *abort_flag);
+  }
+};
 
 // A piece: [rows] pairs (maximum in the log2 domain, sum), then [rows][128] of the output, not divided by the sum.
 template <int ROWS>
@@ -135,11 +231,14 @@ struct Piece {
   __device__ static float* slot(const PagedArgs& a, int cta, int which) { return a.part + (size_t(cta) * 2 + size_t(which)) * kFloats; }
 };
 
-// What the call's first kernel does: the status is good, rows behind the last request are zeros.
+// What the call's first kernel does beside its own work.  At its start: the status is good.
+__device__ __forceinline__ void reset_status(const PagedArgs& a) {
+  if (a.leads && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+}
+// At its end, all threads: rows behind the last request are zeros.
 template <typename T>
-__device__ __forceinline__ void lead(const PagedArgs& a) {
+__device__ __forceinline__ void zero_tail(const PagedArgs& a) {
   if (!a.leads) return;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
   const int tail = min(max(a.cu_new[a.requests], 0), a.rows), vectors = a.hq * kAttnD / 8;
   for (int64_t row = int64_t(tail) + blockIdx.x; row < a.rows; row += gridDim.x)
     for (int v = int(threadIdx.x); v < vectors; v += int(blockDim.x))
@@ -147,61 +246,70 @@ __device__ __forceinline__ void lead(const PagedArgs& a) {
 }
 
 // ---- the join ---------------------------------------------------------------------------------------------------------
-// Where an item starts in span c and goes on in the next, its pieces are weighted with 2^(maximum - greatest maximum) and added in order.  A
-// row is WARPS warps' work, each takes every WARPS-th piece; kJoinThreads / 32 / WARPS rows a CTA, span blockIdx.x.  `locate(item, row)`: the output row.
+// Where an item starts in span c = blockIdx.x and goes on in the next, its pieces are weighted with 2^(maximum - greatest maximum) and added
+// in order.  Eight rows a CTA: a warp each, or, where there are many pieces, all warps for one row after the other.
 constexpr int kJoinThreads = 256;
-template <typename T, int ROWS, int WARPS, typename Locate>
-__device__ __forceinline__ void join_rows(const PagedArgs& a, int spans, Locate locate) {
-  constexpr int kWarps = kJoinThreads / 32;
-  __shared__ float s_m[kWarps], s_l[kWarps];
-  __shared__ __align__(16) float4 s_o[kWarps][32];
-  const int c = int(blockIdx.x);
-  const int4 here = a.starts[c], next = a.starts[c + 1];
-  if (next.z == 0 || (here.x == next.x && here.y == next.y && here.z > 0)) return;  // nothing starts here that goes on
-  const int warp = int(threadIdx.x >> 5), lane = int(threadIdx.x & 31);
-  const int row = int(blockIdx.y) * (kWarps / WARPS) + warp / WARPS;
-  T* dst = locate(next, row);
-  if (__syncthreads_count(dst != nullptr) == 0) return;
-  int pieces = 1;  // and one in each of the following spans that start inside of the item
-  for (int k0 = c + 1; k0 < spans; k0 += kJoinThreads) {
-    const int k = k0 + int(threadIdx.x);
-    const int4 from = k < spans ? a.starts[k] : make_int4(-1, 0, 0, 0);
-    pieces += __syncthreads_count(from.x == next.x && from.y == next.y && from.z > 0);
-  }
+constexpr int kJoinRows = kJoinThreads / 32;
+constexpr int kJoinMany = 24;  // pieces from which on the warps share a row: rounds of four loads, one after the other
+struct Joined {
   float m = -INFINITY, l = 0;
   float4 o = make_float4(0, 0, 0, 0);
-  if (dst != nullptr) {
+  __device__ __forceinline__ void add(const float2& ml, const float4& v) {
+    const float now = fmaxf(m, ml.x), u = now == -INFINITY ? 0.f : now;
+    const float c0 = exp2_fast(m - u), c1 = exp2_fast(ml.x - u);
+    m = now;
+    l = l * c0 + ml.y * c1;
+    o = make_float4(o.x * c0 + v.x * c1, o.y * c0 + v.y * c1, o.z * c0 + v.z * c1, o.w * c0 + v.w * c1);
+  }
+};
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int spans) {
+  __shared__ float2 s_ml[kJoinRows];
+  __shared__ __align__(16) float4 s_o[kJoinRows][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int c = int(blockIdx.x), warp = int(threadIdx.x >> 5), lane = int(threadIdx.x & 31);
+  const Start here = a.starts[c], next = a.starts[c + 1];
+  int k = c + 2 + int(threadIdx.x);  // where the spans behind start
+  Start from = k <= spans ? a.starts[k] : Start{-1, 0, 0, 0, 0, 0, 0};
+  const int row0 = int(blockIdx.y) * kJoinRows;
+  if (next.tile == 0 || (here.request == next.request && here.number == next.number && here.tile > 0) || row0 >= next.rows) return;
+  int pieces = 2;  // one in this span, and in each of the following ones that start inside of the item
+  for (int base = c + 2; base <= spans; base += kJoinThreads) {
+    pieces += __syncthreads_count(from.request == next.request && from.number == next.number && from.tile > 0);
+    k += kJoinThreads;
+    from = k <= spans ? a.starts[k] : Start{-1, 0, 0, 0, 0, 0, 0};
+  }
+  auto write = [&](const Joined& x, int row) {
+    const float inv = x.l == 0 ? 0.f : 1 / x.l;
+    const int at = next.row0 + row, j = at / a.group;
+    T* dst = static_cast<T*>(a.out) + (next.out_row0 + int64_t(j) * a.hq + (at - j * a.group)) * kAttnD + lane * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x.o.x * inv, x.o.y * inv), pack2<T>(x.o.z * inv, x.o.w * inv));
+  };
+  auto gather = [&](int row, int first, int step) {
+    Joined x;
 #pragma unroll 4
-    for (int n = warp % WARPS; n < pieces; n += WARPS) {
+    for (int n = first; n < pieces; n += step) {
       const float* p = Piece<ROWS>::slot(a, c + n, n == 0 ? 1 : 0);
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + 2 * row));
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + size_t(row) * kAttnD + lane * 4));
-      const float mn = fmaxf(m, ml.x), u = mn == -INFINITY ? 0.f : mn;
-      const float c0 = exp2_fast(m - u), c1 = exp2_fast(ml.x - u);
-      m = mn;
-      l = l * c0 + ml.y * c1;
-      o = make_float4(o.x * c0 + v.x * c1, o.y * c0 + v.y * c1, o.z * c0 + v.z * c1, o.w * c0 + v.w * c1);
+      x.add(__ldcg(reinterpret_cast<const float2*>(p + 2 * row)), __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + size_t(row) * kAttnD + lane * 4)));
     }
+    return x;
+  };
+  if (pieces < kJoinMany) {
+    if (row0 + warp < next.rows) write(gather(row0 + warp, 0, 1), row0 + warp);
+    return;
   }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-  s_o[warp][lane] = o;
-  __syncthreads();
-  if (warp % WARPS == 0 && dst != nullptr) {
-    m = -INFINITY;
-    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_m[warp + w]);
-    l = 0;
-    o = make_float4(0, 0, 0, 0);
-    for (int w = 0; w < WARPS; ++w) {
-      const float x = s_m[warp + w] == -INFINITY ? 0.f : exp2_fast(s_m[warp + w] - m);
-      const float4 v = s_o[warp + w][lane];
-      l += s_l[warp + w] * x;
-      o = make_float4(o.x + v.x * x, o.y + v.y * x, o.z + v.z * x, o.w + v.w * x);
+  for (int row = row0; row < min(row0 + kJoinRows, next.rows); ++row) {
+    const Joined mine = gather(row, warp, kJoinRows);
+    if (lane == 0) s_ml[warp] = make_float2(mine.m, mine.l);
+    s_o[warp][lane] = mine.o;
+    __syncthreads();
+    if (warp == (row & (kJoinRows - 1))) {
+      Joined x;
+      for (int w = 0; w < kJoinRows; ++w) x.add(s_ml[w], s_o[w][lane]);
+      write(x, row);
     }
-    const float inv = l == 0 ? 0.f : 1 / l;
-    *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+    __syncthreads();
   }
 }
 
