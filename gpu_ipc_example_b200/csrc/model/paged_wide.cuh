@@ -10,14 +10,19 @@
 //   warp 11      walks the span, hands out its items and brings their rows of Q
 //
 // Items of more than 128 rows: accumulator w is rows 128 w .. of the item, over the same tiles of positions.  Items of up to 128: both have
-// the same rows, w = 0 the even tiles, w = 1 the odd ones, and are added at the end.  Either way the tensor cores work for one of them while
-// the other's softmax runs.  Tensor memory is full: 2 x 128 columns S (P over it, 16 bits), 2 x 128 columns O.  The running maximum is only
-// moved when it grows by more than 2^8: till then weights are up to 256 instead of 1, which fp32 sums and 16-bit weights hold alike
-// (relative rounding), and O is left alone (fetching and storing it costs as much as the softmax of a tile).  The order of S_w(j + 1)
-// behind O_w(j) in the one issuing thread is what makes both "P has been read" and "O is complete" follow from "S is there".
+// the same rows, w = 0 the even tiles, w = 1 the odd ones, and are added at the end.
 //
-// Bound by the exponentials where rows are many (128 x 128 weights at 16 a clock are 1024 clocks, their two products 1024 on the tensor
-// cores), by memory where they are few.
+// A tile's scores come in two halves of 64 positions, each into columns of its own: while a softmax is at one half, the products of the
+// half before and the scores of the one behind run, so that neither waits for the way there and back (arrival, wait, issue and commit are
+// 350 clocks by themselves; with one buffer of 128 positions the chain of scores, softmax and outputs took 5300 clocks a pair of
+// tiles).  Tensor memory is full: 2 x 2 x 64 columns S (P over its first half, 16 bits), 2 x 128 columns O.  S(i + 2) is issued behind O(i) by the
+// same thread, so "S is there" says that P(i) has been read and O(i) added.
+//
+// The running maximum is only moved when it grows by more than 2^8: till then weights are up to 256 instead of 1, which fp32 sums and
+// 16-bit weights hold alike (relative rounding), and O is left alone.
+//
+// Bound by the exponentials (128 x 128 weights at 16 a clock are 1024 clocks) and the tensor cores (1280: 512 for the outputs, 768 for the
+// scores, whose operands both come from shared memory) where rows are many, by memory where they are few.
 #pragma once
 
 #include "paged_work.cuh"
@@ -26,9 +31,9 @@ namespace b200ipc {
 
 constexpr int kWideRows = 256;
 constexpr int kWideTile = 128;   // positions
+constexpr int kWideHalf = 64;
 constexpr int kWideStages = 4;   // K or V tiles
 constexpr int kWideThreads = 384;  // three warpgroups
-constexpr int kWideRegsSoftmax = 208, kWideRegsRest = 88;  // 256 x 208 + 128 x 88 = 384 x 168, what the launch has
 constexpr int kWideTileBytes = kWideTile * kAttnD * 2;  // also of 128 rows of Q
 constexpr int kWideStage = 4096;  // bytes of a softmax warp's way out: 32 rows x 128
 constexpr size_t kWideSmem = 1024 + size_t(kWideStages + 2) * kWideTileBytes + 8 * kWideStage;
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   extern __shared__ unsigned char smem_raw[];
   using Items = Queue<WideItem, 11>;  // the softmax warps, the stream, the products
   __shared__ Items s_queue;
-  __shared__ uint64_t kv_full[kWideStages], kv_empty[kWideStages], q_ready[2], q_free[2], s_full[2], p_ready[2][2], o_full[2], mma_done;
+  __shared__ uint64_t kv_full[kWideStages], kv_empty[kWideStages], q_ready[2], q_free[2], s_full[2][2], p_ready[2][2], o_late[2], o_full[2], mma_done;
   __shared__ float2 s_ml[128];  // maxima and sums of w = 1
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -233,7 +238,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
     for (int w = 0; w < 2; ++w) {
       mbar_init(&q_ready[w], 1);
       mbar_init(&q_free[w], 2);
-      mbar_init(&s_full[w], 1);
+      mbar_init(&s_full[w][0], 1);
+      mbar_init(&s_full[w][1], 1);
+      mbar_init(&o_late[w], 1);
       mbar_init(&p_ready[w][0], 4);  // a warp is one arrival: 128 on one word would stand in line
       mbar_init(&p_ready[w][1], 4);
       mbar_init(&o_full[w], 1);
@@ -260,12 +267,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   auto wait = [&](uint64_t* bar, uint32_t parity) { items.wait(bar, parity); };
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegsSoftmax));
     // ---- softmax: thread = row of the accumulator -----------------------------------------------------------------------
     const int w = warp >> 2, row = (warp & 3) * 32 + lane, G = args.group;
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t s_addr = lane_base + uint32_t(w) * 128u, o_addr = lane_base + 256u + uint32_t(w) * 128u;
-    uint32_t ph_s = 0, ph_o = 0, ring_at = 0, ring_ph = 0;  // the ring position of the item's first tile
+    uint32_t ph_s = 0, ph_o = 0, ring_at = 0, ring_ph = 0;  // ring_at: the ring position of the item's first tile
     for (const WideItem* x = items.take(); x != nullptr; x = items.take()) {
       // What is needed once is read or computed again: the loop over the tiles has few registers to spare.
       const int count = x->count[w], G0 = x->split ? 0 : w * 128;  // first row of this accumulator in the item
@@ -274,13 +280,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         const bool busy = G0 + (warp & 3) * 32 < x->rows;  // this warp has rows
         // positions that this row sees
         const int limit = G0 + row < x->rows ? x->len - x->n + (x->row0 + G0 + row) / G + 1 : 0;
+        const int tile_step = x->split ? 2 * kWideTile - kWideHalf : kWideHalf;  // from a tile's second half to the next tile
         int p0 = (x->t0 + (x->split ? w : 0)) * kWideTile;
-        for (int t = 0; t < count; ++t, p0 += x->split ? 2 * kWideTile : kWideTile) {
-          wait(&s_full[w], ph_s);
-          ph_s ^= 1u;
+        for (int i = 0; i < 2 * count; ++i, p0 += i & 1 ? kWideHalf : tile_step) {
+          const int b = i & 1;
+          wait(&s_full[w][b], ph_s);
           // Values of positions that do not exist count as zero (a weight of zero would not do: they may be NaN).  They are in the item's last
           // tile; each softmax that uses it clears them, as neither waits for the other.
-          if (t == count - 1 && x->t1 * kWideTile > x->len) {
+          if (i == 2 * count - 2 && x->t1 * kWideTile > x->len) {
             const int n = x->t1 - x->t0;
             if (x->split ? ((n - 1) & 1) == w : count == n) {
               const uint32_t v_at = ring_at + uint32_t(2 * n - 1);  // that tile in the ring
@@ -297,99 +304,73 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
               fence_async_smem();
             }
           }
-          auto half_done = [&](int half) {  // 64 positions' weights are there
-            if (busy) {
-              tmem_st_wait();
-              tc_fence_before_sync();
+          if (busy) {
+            tc_fence_after_sync();
+            const uint32_t s_at = s_addr + uint32_t(b) * kWideHalf;
+            float s[kWideHalf];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_ld_32cols(s_at + uint32_t(c) * 32u, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+            tmem_ld_wait();
+            if (__any_sync(0xffffffffu, limit < p0 + kWideHalf)) {
+#pragma unroll
+              for (int e = 0; e < kWideHalf; ++e)
+                if (p0 + e >= limit) s[e] = -INFINITY;
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[w][half]);
-          };
-          if (!busy) {
-            half_done(0);
-            half_done(1);
-            continue;
-          }
-          tc_fence_after_sync();
-          // All 128 columns for the maximum.  The second half of them is fetched once more for the weights, 32 at a time behind the first
-          // half's: 64 registers less.
-          float s[4][32];
-          auto fetch_s = [&](int c) { tmem_ld_32cols(s_addr + uint32_t(c) * 32u, *reinterpret_cast<uint32_t(*)[32]>(&s[c][0])); };
-          const bool masked = __any_sync(0xffffffffu, limit < p0 + kWideTile);
-          auto mask = [&](int c) {
-            if (masked) {
+            float mx[4];
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (p0 + 32 * c + e >= limit) s[c][e] = -INFINITY;
-            }
-          };
+            for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[e + 4], s[e + 8]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) fetch_s(c);
-          tmem_ld_wait();
+            for (int e = 12; e < kWideHalf; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], s[e], s[e + 1]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * args.scale_log2;
+            if (__any_sync(0xffffffffu, top > ref + kWideSlack)) {
+              const float now = fmaxf(ref, top);
+              if (i > 0) {
+                // O(i - 1) has to be there: what says so is S(i + 1), or, for the last one, a word of its own
+                if (i + 1 < 2 * count) wait(&s_full[w][b ^ 1], b ? ph_s ^ 1u : ph_s);
+                else wait(&o_late[w], ph_o);
+                tc_fence_after_sync();
+                const float f = now == -INFINITY ? 1.f : exp2_fast(ref - now);
+                sum *= f;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mask(c);
-          float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+                for (int c = 0; c < 8; ++c) {
+                  uint32_t o[16];
+                  tmem_ld_16cols(o_addr + uint32_t(c) * 16u, o);
+                  tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], s[c][e], s[c][e + 1]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * args.scale_log2;
-          if (__any_sync(0xffffffffu, top > ref + kWideSlack)) {
-            const float now = fmaxf(ref, top);
-            if (t > 0) {
-              const float f = now == -INFINITY ? 1.f : exp2_fast(ref - now);
-              sum *= f;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                uint32_t o[16];
-                tmem_ld_16cols(o_addr + uint32_t(c) * 16u, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st_16cols(o_addr + uint32_t(c) * 16u, o);
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st_16cols(o_addr + uint32_t(c) * 16u, o);
+                }
               }
+              ref = now;
             }
-            ref = now;
-          }
-          const float shift = ref == -INFINITY ? 0.f : -ref;
-          uint64_t part[2] = {0, 0};  // pairs of sums
-          auto weights = [&](int c) {  // 32 positions from 32 c on
-            uint32_t p[16];
+            const float shift = ref == -INFINITY ? 0.f : -ref;
+            uint64_t part[2] = {0, 0};  // pairs of sums
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint64_t v = f32x2_fma(f32x2(s[c][2 * e], s[c][2 * e + 1]), f32x2(args.scale_log2, args.scale_log2), f32x2(shift, shift));
-              float2 y = f32x2_parts(v);
-              y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-              part[e & 1] = f32x2_add(part[e & 1], f32x2(y.x, y.y));
-              p[e] = pack2<T>(y.x, y.y);
+            for (int c = 0; c < 2; ++c) {
+              uint32_t p[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float2 y = f32x2_parts(f32x2_fma(f32x2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), f32x2(args.scale_log2, args.scale_log2), f32x2(shift, shift)));
+                y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                part[e & 1] = f32x2_add(part[e & 1], f32x2(y.x, y.y));
+                p[e] = pack2<T>(y.x, y.y);
+              }
+              tmem_st_16cols(s_at + uint32_t(c) * 16u, p);
             }
-            tmem_st_16cols(s_addr + uint32_t(c) * 16u, p);  // over columns that are not needed any more
-          };
-          weights(0);
-          fetch_s(2);
-          weights(1);
-          half_done(0);
-          tmem_ld_wait();
-          fetch_s(3);
-          mask(2);
-          weights(2);
-          tmem_ld_wait();
-          mask(3);
-          weights(3);
-          half_done(1);
-          const float2 a = f32x2_parts(f32x2_add(part[0], part[1]));
-          sum += a.x + a.y;
+            tmem_st_wait();
+            tc_fence_before_sync();
+            const float2 a = f32x2_parts(f32x2_add(part[0], part[1]));
+            sum += a.x + a.y;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[w][b]);
+          ph_s ^= uint32_t(b);
         }
       }
       // ---- the end of the item ---------------------------------------------------------------------------------------------------
       const bool split = x->split != 0, whole = x->whole != 0, both = split && x->t1 - x->t0 > 1;
       const bool busy = G0 + (warp & 3) * 32 < x->rows, exists = G0 + row < x->rows;
       const int at = x->row0 + G0 + row, j = at / G;
-      // a row that sees nothing of this accumulator's positions (it sees the first so many)
-      if (!exists || x->len - x->n + j + 1 <= (x->t0 + (split ? w : 0)) * kWideTile) {
-        ref = -INFINITY;
-        sum = 0;
-      }
       if (count > 0) {
         wait(&o_full[w], ph_o);
         ph_o ^= 1u;
@@ -479,9 +460,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       items.give_back();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsRest));
     if (warp == 8) {
-      // ---- the stream: K(0), then K(j + 1) and V(j) in turn.  Lane l knows where box l of a tile is. ------------------------
+      // ---- the stream: K and V of a tile after the other.  Lane l knows where box l of it is. -------------------------------
       const int box = min(args.page, 64), boxes = kWideTile / box, per_page = args.page / box;
       const int outside = int(args.pages * args.hkv * args.page);
       uint32_t st = 0, ph = 0;
@@ -508,24 +488,19 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       };
       for (const WideItem* x = items.take(); x != nullptr; x = items.take()) {
         const int* table = args.table + int64_t(x->request) * args.width;
-        const int len = x->len, h = x->h, t0 = x->t0, t1 = x->t1, pages = (len + args.page - 1) / args.page;
-        int base = -64, entry = 0, at = 0, n = 0;  // the tile whose V comes next
-        for (int t = t0; t <= t1 && t1 > t0; ++t) {
-          int k_at = 0, k_n = 0;
-          if (t < t1) {
-            const int b = t * boxes + (lane & (boxes - 1)), p = b / per_page;
-            if ((t * boxes + boxes - 1) / per_page >= base + 32) {
-              base = t * boxes / per_page;
-              entry = base + lane < pages ? table[base + lane] : -1;
-            }
-            const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
-            k_at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
-            k_n = min(boxes, (len - t * kWideTile + box - 1) / box);  // boxes that hold positions of the request
-            load(&args.tma_k, k_at, k_n);
+        const int len = x->len, h = x->h, t1 = x->t1, pages = (len + args.page - 1) / args.page;
+        int base = -64, entry = 0;  // 32 entries of the request's table, one per lane
+        for (int t = x->t0; t < t1; ++t) {
+          const int b = t * boxes + (lane & (boxes - 1)), p = b / per_page;
+          if ((t * boxes + boxes - 1) / per_page >= base + 32) {
+            base = t * boxes / per_page;
+            entry = base + lane < pages ? table[base + lane] : -1;
           }
-          if (t > t0) load(&args.tma_v, at, n);
-          at = k_at;
-          n = k_n;
+          const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
+          const int at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
+          const int n = min(boxes, (len - t * kWideTile + box - 1) / box);  // boxes that hold positions of the request
+          load(&args.tma_k, at, n);
+          load(&args.tma_v, at, n);
         }
         items.give_back();
       }
@@ -536,7 +511,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       // ---- the products of accumulator w: one thread ---------------------------------------------------------------------------
       if (elect_one()) {
         const int w = warp - 9;
-        const uint32_t idesc_s = make_idesc<T>(128, kWideTile), idesc_o = make_idesc<T>(128, kAttnD) | (1u << 16);
+        const uint32_t idesc_s = make_idesc<T>(128, kWideHalf), idesc_o = make_idesc<T>(128, kAttnD) | (1u << 16);
         const uint32_t t_s = tmem + uint32_t(w) * 128u, t_o = t_s + 256u;
         // 64 columns of a K-major tile are one block of it, 16 of them 32 bytes of its rows; descriptors count in 16 bytes
         const uint64_t q_desc = make_sw128_kmajor_desc(smem_u32(q_smem)), k_desc = make_sw128_kmajor_desc(smem_u32(ring)), v_desc = make_sw128_nmajor_desc(smem_u32(ring));
@@ -555,29 +530,22 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         // a wait for a stage's next round must come from who has seen the round before, and find the round it waits for still there.  The
         // same with Q.
         auto landed = [&](const Place& p) { wait(&kv_full[p.st], p.ph); };
-        auto scores = [&](uint64_t q, const Place& p) {
-          tc_fence_after_sync();
-          const uint64_t k = k_desc + uint64_t(p.st) * kTileStep;
+        auto scores = [&](uint64_t q, const Place& p, int b) {  // of half b of a tile
+          const uint64_t k = k_desc + uint64_t(p.st) * kTileStep + uint64_t(b) * (kWideHalf * 128 / 16);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint64_t o = uint64_t(i >> 2) * kBlockStep + uint64_t(i & 3) * 2u;
-            umma_f16(t_s, q + o, k + o, idesc_s, i > 0 ? 1u : 0u);
+            umma_f16(t_s + uint32_t(b) * kWideHalf, q + o, k + o, idesc_s, i > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[w]);
+          umma_commit(&s_full[w][b]);
         };
-        auto outputs = [&](bool fresh, const Place& p) {  // in two halves, as P comes
+        auto outputs = [&](bool fresh, const Place& p, int b) {
           const uint64_t v = v_desc + uint64_t(p.st) * kTileStep;
+          wait(&p_ready[w][b], ph_p);
+          tc_fence_after_sync();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            wait(&p_ready[w][half], ph_p);
-            tc_fence_after_sync();
-#pragma unroll
-            for (int i = 0; i < kWideTile / 32; ++i) {  // 16 positions: 8 columns of P, 2048 bytes of V
-              const int k = half * (kWideTile / 32) + i;
-              umma_f16_ts(t_o, t_s + uint32_t(k * 8), v + uint64_t(k) * 128u, idesc_o, !fresh || k > 0 ? 1u : 0u);
-            }
-          }
-          ph_p ^= 1u;
+          for (int i = 0; i < kWideHalf / 16; ++i)  // 16 positions: 8 columns of P, 2048 bytes of V
+            umma_f16_ts(t_o, t_s + uint32_t(b * kWideHalf + i * 8), v + uint64_t(b * (kWideHalf / 16) + i) * 128u, idesc_o, !fresh || i > 0 ? 1u : 0u);
         };
         for (const WideItem* x = items.take_alone(); x != nullptr; x = items.take_alone()) {
           const int n = x->t1 - x->t0, count = x->count[w];
@@ -591,49 +559,64 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
           mbar_arrive(&q_free[split ? 1 : 1 - w]);  // what is not used or the other's
           const uint64_t q = q_desc + uint64_t(split ? 0 : w) * kTileStep;
           uint64_t* q_done = &q_free[split ? 0 : w];
-          int scored = 0, done = 0;  // tiles whose S, whose O has been issued
-          auto score = [&](const Place& p) {
-            scores(q, p);
-            if (++scored == count) umma_commit(q_done);
+          // The ring has K and V of a tile after the other.  Those of tiles that are not this accumulator's (split: every other one; else the
+          // last ones, which its rows do not see) are given back unread.
+          auto give_up = [&]() {
+            const Place p = next();
+            landed(p);
+            mbar_arrive(&kv_empty[p.st]);
           };
-          auto output = [&](const Place& p) {
-            outputs(done == 0, p);
-            if (++done == count) umma_commit(&o_full[w]);
-          };
+          int passed = 0;  // tiles of the ring that have been taken
           if (count == 0) mbar_arrive(q_done);
-          // The ring has K(0), then K(j + 1) and V(j) in turn.  `mine`: this accumulator looks at tile j.
-          auto mine = [&](int j) { return split ? (j & 1) == w : j < count; };
-          auto release = [&](const Place& p, bool used) {
-            if (used) umma_commit(&kv_empty[p.st]);
-            else mbar_arrive(&kv_empty[p.st]);
-          };
-          if (n > 0) {
-            const Place k = next();
-            landed(k);
-            if (mine(0)) score(k);
-            release(k, mine(0));
-          }
-          for (int j = 0; j < n; ++j) {
-            const bool more = j + 1 < n;
-            const Place k = more ? next() : at, v = next();
-            if (more) landed(k);
-            if (split) {  // K(j + 1) and V(j) are not the same one's
-              if (more) {
-                if (mine(j + 1)) score(k);
-                release(k, mine(j + 1));
-              }
-              landed(v);
-              if (mine(j)) output(v);
-              release(v, mine(j));
-            } else {  // P(j) has to be read before S(j + 1) goes over it
-              landed(v);
-              if (mine(j)) output(v);
-              release(v, mine(j));
-              if (more) {
-                if (mine(j + 1)) score(k);
-                release(k, mine(j + 1));
-              }
+          if (count > 0) {
+            if (split && w == 1) {
+              give_up();
+              give_up();
+              passed = 1;
             }
+            Place k = next(), v = next();
+            ++passed;
+            landed(k);
+            scores(q, k, 0);
+            scores(q, k, 1);
+            umma_commit(&kv_empty[k.st]);
+            if (count == 1) umma_commit(q_done);
+            for (int t = 0; t < count; ++t) {
+              const bool more = t + 1 < count;
+              landed(v);
+              outputs(t == 0, v, 0);
+              Place k1 = k, v1 = v;
+              if (more) {
+                if (split) {
+                  give_up();
+                  give_up();
+                  ++passed;
+                }
+                k1 = next();
+                v1 = next();
+                ++passed;
+                landed(k1);
+                scores(q, k1, 0);
+              } else {
+                umma_commit(&o_late[w]);
+              }
+              outputs(false, v, 1);
+              umma_commit(&kv_empty[v.st]);
+              if (more) {
+                scores(q, k1, 1);
+                umma_commit(&kv_empty[k1.st]);
+                if (t + 2 == count) umma_commit(q_done);  // behind its last reader
+              } else {
+                umma_commit(&o_full[w]);
+              }
+              ph_p ^= 1u;
+              k = k1;
+              v = v1;
+            }
+          }
+          for (; passed < n; ++passed) {
+            give_up();
+            give_up();
           }
           items.give_back_alone();
         }

@@ -182,7 +182,7 @@ struct QueueEnd {
   volatile int* abort_flag;
   uint32_t at = 0, ph = 0;
   __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
-    if (!mbar_try_wait(bar, parity) && !*abort_flag) mbar_wait_long(bar, parity, abort_flag, kPagedTimeoutNs);
+    if (!mbar_try_wait(bar, parity) && !*abort_flag) mbar_wait(bar, parity, abort_flag, kPagedTimeoutNs);
   }
   __device__ __forceinline__ void step() {
     if (++at == kPagedQueue) {
