@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
         const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
         const int at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
         const int n = min(boxes, (len - t * kNarTile + box - 1) / box);  // boxes that hold positions of the request
-        items.wait(&empty[st], ph ^ 1u);
+        items.wait_warp(&empty[st], ph ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
         if (lane == 0) mbar_expect_tx(&full[st], uint32_t(n * box) * kAttnD * 4u);
         __syncwarp();
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
       for (int d = 0; d < 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0;
       for (int t = t0; t < t1; ++t) {
         if (int(st & 1u) == side) {
-          items.wait(&full[st], ph);
+          items.wait_warp(&full[st], ph);
           const uint32_t kt = ring_addr + st * 2 * kNarTileBytes, vt = kt + kNarTileBytes;
           const int pos = t * kNarTile + at;
           if (pos < len) {

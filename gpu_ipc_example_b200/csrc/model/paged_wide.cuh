@@ -10,9 +10,9 @@
 //   warp 11      walks the span, hands out its items and brings their rows of Q
 //
 // Items of more than 128 rows: accumulator w is rows 128 w .. of the item, over the same tiles of positions.  Items of up to 128: both have
-// the same rows, w = 0 the even tiles, w = 1 the odd ones, and are added at the end.
+// the same rows, accumulator w the w-th half of every tile, and are added at the end.
 //
-// A tile's scores come in two halves of 64 positions, each into columns of its own: while a softmax is at one half, the products of the
+// Scores come by halves of a tile, 64 positions, into two sets of columns in turn: while a softmax is at one half, the products of the
 // half before and the scores of the one behind run, so that neither waits for the way there and back (arrival, wait, issue and commit are
 // 350 clocks by themselves; with one buffer of 128 positions the chain of scores, softmax and outputs took 5300 clocks a pair of
 // tiles).  Tensor memory is full: 2 x 2 x 64 columns S (P over its first half, 16 bits), 2 x 128 columns O.  S(i + 2) is issued behind O(i) by the
@@ -48,8 +48,8 @@ struct WideItem {
   int first, n, len;    // the request's first row of q, its new tokens, its tokens in the cache
   int row0, rows;       // rows of the item within the request
   int t0, t1, whole;    // tiles of positions; whether these are all
-  int split;            // up to 128 rows: the accumulators take tiles in turn
-  int count[2];         // tiles that accumulator w looks at: from t0 on, or every other one
+  int split;            // up to 128 rows: the accumulators take a half of every tile each
+  int count[2];         // halves of tiles that accumulator w looks at
 };
 
 struct WideCut {
@@ -133,10 +133,10 @@ struct WideWalk {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       if (x.split) {
-        x.count[w] = (x.t1 - x.t0 + 1 - w) / 2;
+        x.count[w] = x.t1 - x.t0;
       } else {
         const int see = cut.seen(r, x.row0 + min(x.rows, (w + 1) * 128));
-        x.count[w] = max(0, min((see + kWideTile - 1) / kWideTile, x.t1) - x.t0);
+        x.count[w] = 2 * max(0, min((see + kWideTile - 1) / kWideTile, x.t1) - x.t0);
       }
     }
     t0 = 0;
@@ -265,13 +265,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   const uint32_t tmem = s_tmem;
   QueueEnd<Items, WideItem> items{s_queue, abort_flag};
   auto wait = [&](uint64_t* bar, uint32_t parity) { items.wait(bar, parity); };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { items.wait_warp(bar, parity); };
 
   if (warp < 8) {
     // ---- softmax: thread = row of the accumulator -----------------------------------------------------------------------
     const int w = warp >> 2, row = (warp & 3) * 32 + lane, G = args.group;
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t s_addr = lane_base + uint32_t(w) * 128u, o_addr = lane_base + 256u + uint32_t(w) * 128u;
-    uint32_t ph_s = 0, ph_o = 0, ring_at = 0, ring_ph = 0;  // ring_at: the ring position of the item's first tile
+    uint32_t part_no = 0, ph_o = 0, ring_at = 0;  // halves of tiles so far, and the ring's tiles before the item
     for (const WideItem* x = items.take(); x != nullptr; x = items.take()) {
       // What is needed once is read or computed again: the loop over the tiles has few registers to spare.
       const int count = x->count[w], G0 = x->split ? 0 : w * 128;  // first row of this accumulator in the item
@@ -280,33 +281,28 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         const bool busy = G0 + (warp & 3) * 32 < x->rows;  // this warp has rows
         // positions that this row sees
         const int limit = G0 + row < x->rows ? x->len - x->n + (x->row0 + G0 + row) / G + 1 : 0;
-        const int tile_step = x->split ? 2 * kWideTile - kWideHalf : kWideHalf;  // from a tile's second half to the next tile
-        int p0 = (x->t0 + (x->split ? w : 0)) * kWideTile;
-        for (int i = 0; i < 2 * count; ++i, p0 += i & 1 ? kWideHalf : tile_step) {
-          const int b = i & 1;
-          wait(&s_full[w][b], ph_s);
+        const int step = x->split ? kWideTile : kWideHalf;
+        int p0 = x->t0 * kWideTile + (x->split ? w * kWideHalf : 0);
+        for (int i = 0; i < count; ++i, p0 += step) {
+          const uint32_t b = part_no & 1u;
+          wait_warp(&s_full[w][b], (part_no >> 1) & 1u);
+          ++part_no;
           // Values of positions that do not exist count as zero (a weight of zero would not do: they may be NaN).  They are in the item's last
           // tile; each softmax that uses it clears them, as neither waits for the other.
-          if (i == 2 * count - 2 && x->t1 * kWideTile > x->len) {
-            const int n = x->t1 - x->t0;
-            if (x->split ? ((n - 1) & 1) == w : count == n) {
-              const uint32_t v_at = ring_at + uint32_t(2 * n - 1);  // that tile in the ring
-              const uint32_t v_st = v_at % kWideStages, v_ph = ring_ph ^ ((v_at / kWideStages) & 1u);
-              wait(&kv_full[v_st], v_ph);
-              if (p0 + row >= x->len) {
-                unsigned char* v = ring + v_st * kWideTileBytes + row * 128;
-#pragma unroll 4
-                for (int c = 0; c < 8; ++c) {
-                  *reinterpret_cast<uint4*>(v + (c << 4)) = make_uint4(0, 0, 0, 0);
-                  *reinterpret_cast<uint4*>(v + kWideTileBytes / 2 + (c << 4)) = make_uint4(0, 0, 0, 0);
-                }
-              }
-              fence_async_smem();
+          if (p0 + kWideHalf > x->len) {
+            const uint32_t v_at = ring_at + uint32_t(2 * (x->t1 - x->t0) - 1), v_st = v_at % kWideStages;  // that tile in the ring
+            wait_warp(&kv_full[v_st], (v_at / kWideStages) & 1u);
+            const int at = row & (kWideHalf - 1), first = p0 & (kWideTile - 1);  // two threads a position, half of its dimensions each
+            if (p0 + at >= x->len) {
+              unsigned char* v = ring + v_st * kWideTileBytes + (first + at) * 128 + (row >= kWideHalf ? kWideTileBytes / 2 : 0);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + (c << 4)) = make_uint4(0, 0, 0, 0);
             }
+            fence_async_smem();
           }
           if (busy) {
             tc_fence_after_sync();
-            const uint32_t s_at = s_addr + uint32_t(b) * kWideHalf;
+            const uint32_t s_at = s_addr + b * kWideHalf;
             float s[kWideHalf];
 #pragma unroll
             for (int c = 0; c < 2; ++c) tmem_ld_32cols(s_at + uint32_t(c) * 32u, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
@@ -326,8 +322,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
               const float now = fmaxf(ref, top);
               if (i > 0) {
                 // O(i - 1) has to be there: what says so is S(i + 1), or, for the last one, a word of its own
-                if (i + 1 < 2 * count) wait(&s_full[w][b ^ 1], b ? ph_s ^ 1u : ph_s);
-                else wait(&o_late[w], ph_o);
+                if (i + 1 < count) wait_warp(&s_full[w][b ^ 1u], (part_no >> 1) & 1u);
+                else wait_warp(&o_late[w], ph_o);
                 tc_fence_after_sync();
                 const float f = now == -INFINITY ? 1.f : exp2_fast(ref - now);
                 sum *= f;
@@ -364,15 +360,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_ready[w][b]);
-          ph_s ^= uint32_t(b);
         }
       }
       // ---- the end of the item ---------------------------------------------------------------------------------------------------
-      const bool split = x->split != 0, whole = x->whole != 0, both = split && x->t1 - x->t0 > 1;
+      const bool split = x->split != 0, whole = x->whole != 0, both = split && x->t1 > x->t0;
       const bool busy = G0 + (warp & 3) * 32 < x->rows, exists = G0 + row < x->rows;
       const int at = x->row0 + G0 + row, j = at / G;
       if (count > 0) {
-        wait(&o_full[w], ph_o);
+        wait_warp(&o_full[w], ph_o);
         ph_o ^= 1u;
         tc_fence_after_sync();
       }
@@ -454,9 +449,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       }
       tc_fence_before_sync();  // O may be written again once this thread's next weights are there
       if (both) wide_sync();   // of w = 1 as well
-      const uint32_t moved = ring_at + uint32_t(2 * (x->t1 - x->t0));
-      ring_ph ^= (moved / kWideStages) & 1u;
-      ring_at = moved % kWideStages;
+      ring_at += uint32_t(2 * (x->t1 - x->t0));
       items.give_back();
     }
   } else {
@@ -467,7 +460,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       uint32_t st = 0, ph = 0;
       int issued = 0;
       auto load = [&](const CUtensorMap* map, int at, int n) {
-        wait(&kv_empty[st], ph ^ 1u);
+        wait_warp(&kv_empty[st], ph ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) return;
         if (lane == 0) mbar_expect_tx(&kv_full[st], uint32_t(n * box) * kAttnD * 2u);
         __syncwarp();
@@ -516,108 +509,78 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         // 64 columns of a K-major tile are one block of it, 16 of them 32 bytes of its rows; descriptors count in 16 bytes
         const uint64_t q_desc = make_sw128_kmajor_desc(smem_u32(q_smem)), k_desc = make_sw128_kmajor_desc(smem_u32(ring)), v_desc = make_sw128_nmajor_desc(smem_u32(ring));
         constexpr uint64_t kTileStep = kWideTileBytes >> 4, kBlockStep = kWideTileBytes >> 5;
-        struct Place {
-          uint32_t st, ph;
-        };
-        Place at{0, 0};  // the ring's next tile
-        auto next = [&]() {
-          const Place p = at;
-          if (++at.st == kWideStages) at = Place{0, at.ph ^ 1u};
-          return p;
-        };
-        uint32_t ph_q0 = 0, ph_q1 = 0, ph_p = 0;
-        // Both threads wait for every tile, in order, and both have to give it back, also where only one uses it: copies land out of order, and
-        // a wait for a stage's next round must come from who has seen the round before, and find the round it waits for still there.  The
-        // same with Q.
-        auto landed = [&](const Place& p) { wait(&kv_full[p.st], p.ph); };
-        auto scores = [&](uint64_t q, const Place& p, int b) {  // of half b of a tile
-          const uint64_t k = k_desc + uint64_t(p.st) * kTileStep + uint64_t(b) * (kWideHalf * 128 / 16);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint64_t o = uint64_t(i >> 2) * kBlockStep + uint64_t(i & 3) * 2u;
-            umma_f16(t_s + uint32_t(b) * kWideHalf, q + o, k + o, idesc_s, i > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[w][b]);
-        };
-        auto outputs = [&](bool fresh, const Place& p, int b) {
-          const uint64_t v = v_desc + uint64_t(p.st) * kTileStep;
-          wait(&p_ready[w][b], ph_p);
-          tc_fence_after_sync();
-#pragma unroll
-          for (int i = 0; i < kWideHalf / 16; ++i)  // 16 positions: 8 columns of P, 2048 bytes of V
-            umma_f16_ts(t_o, t_s + uint32_t(b * kWideHalf + i * 8), v + uint64_t(b * (kWideHalf / 16) + i) * 128u, idesc_o, !fresh || i > 0 ? 1u : 0u);
-        };
+        uint32_t ph_q0 = 0, ph_q1 = 0;
+        uint32_t base = 0, seen = 0;     // tiles of the ring before the item, and those that have landed
+        uint32_t scored = 0, added = 0;  // halves of tiles whose S, whose O has been issued
         for (const WideItem* x = items.take_alone(); x != nullptr; x = items.take_alone()) {
-          const int n = x->t1 - x->t0, count = x->count[w];
+          const uint32_t end = base + 2u * uint32_t(x->t1 - x->t0), last = added + uint32_t(x->count[w]), first = added;
           const bool split = x->split != 0;
+          const uint32_t shift = split ? 0u : 1u;  // two halves of a tile, or one
           wait(&q_ready[0], ph_q0);
           ph_q0 ^= 1u;
           if (!split) {
             wait(&q_ready[1], ph_q1);
             ph_q1 ^= 1u;
+            mbar_arrive(&q_free[1 - w]);  // the other's, seen
           }
-          mbar_arrive(&q_free[split ? 1 : 1 - w]);  // what is not used or the other's
           const uint64_t q = q_desc + uint64_t(split ? 0 : w) * kTileStep;
           uint64_t* q_done = &q_free[split ? 0 : w];
-          // The ring has K and V of a tile after the other.  Those of tiles that are not this accumulator's (split: every other one; else the
-          // last ones, which its rows do not see) are given back unread.
-          auto give_up = [&]() {
-            const Place p = next();
-            landed(p);
-            mbar_arrive(&kv_empty[p.st]);
-          };
-          int passed = 0;  // tiles of the ring that have been taken
-          if (count == 0) mbar_arrive(q_done);
-          if (count > 0) {
-            if (split && w == 1) {
-              give_up();
-              give_up();
-              passed = 1;
+          if (first == last) mbar_arrive(q_done);
+          // The ring has K and V of a tile after the other.  Scores are issued up to two halves ahead of the outputs, as soon as K is there; outputs
+          // as soon as V and the weights are.  (One after the other in a fixed order, a wait for the next K held up what frees the ring for it.)
+          // Both threads look for every tile in order, and both give it back, also where only one uses it: copies land out of order, and a wait
+          // for a stage's next round must come from who has seen the round before, and find the round it looks for still there.
+          uint64_t since = 0;
+          uint32_t idle = 0;
+          while (added < last || seen < end) {
+            ++idle;
+            if (seen < end && mbar_try_wait(&kv_full[seen % kWideStages], (seen / kWideStages) & 1u, 0)) {
+              if (((seen - base) >> 1) >= ((last - first) >> shift)) mbar_arrive(&kv_empty[seen % kWideStages]);  // not this accumulator's
+              ++seen;
+              idle = 0;
             }
-            Place k = next(), v = next();
-            ++passed;
-            landed(k);
-            scores(q, k, 0);
-            scores(q, k, 1);
-            umma_commit(&kv_empty[k.st]);
-            if (count == 1) umma_commit(q_done);
-            for (int t = 0; t < count; ++t) {
-              const bool more = t + 1 < count;
-              landed(v);
-              outputs(t == 0, v, 0);
-              Place k1 = k, v1 = v;
-              if (more) {
-                if (split) {
-                  give_up();
-                  give_up();
-                  ++passed;
+            if (scored < last && scored < added + 2) {
+              const uint32_t tile = (scored - first) >> shift, k_at = base + 2 * tile;
+              if (seen > k_at) {
+                const uint32_t b = scored & 1u, half = split ? uint32_t(w) : (scored - first) & 1u;
+                const uint64_t k = k_desc + uint64_t(k_at % kWideStages) * kTileStep + uint64_t(half) * (kWideHalf * 128 / 16);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const uint64_t o = uint64_t(i >> 2) * kBlockStep + uint64_t(i & 3) * 2u;
+                  umma_f16(t_s + b * kWideHalf, q + o, k + o, idesc_s, i > 0 ? 1u : 0u);
                 }
-                k1 = next();
-                v1 = next();
-                ++passed;
-                landed(k1);
-                scores(q, k1, 0);
-              } else {
-                umma_commit(&o_late[w]);
+                umma_commit(&s_full[w][b]);
+                if (split || half == 1) umma_commit(&kv_empty[k_at % kWideStages]);
+                if (++scored == last) umma_commit(q_done);  // behind its last reader
+                idle = 0;
               }
-              outputs(false, v, 1);
-              umma_commit(&kv_empty[v.st]);
-              if (more) {
-                scores(q, k1, 1);
-                umma_commit(&kv_empty[k1.st]);
-                if (t + 2 == count) umma_commit(q_done);  // behind its last reader
-              } else {
-                umma_commit(&o_full[w]);
+            }
+            if (added < scored) {
+              const uint32_t tile = (added - first) >> shift, v_at = base + 2 * tile + 1, b = added & 1u;
+              if (seen > v_at && mbar_try_wait(&p_ready[w][b], (added >> 1) & 1u, 0)) {
+                const uint32_t half = split ? uint32_t(w) : (added - first) & 1u;
+                const uint64_t v = v_desc + uint64_t(v_at % kWideStages) * kTileStep + uint64_t(half) * (kWideHalf / 16 * 128);
+                tc_fence_after_sync();
+#pragma unroll
+                for (int i = 0; i < kWideHalf / 16; ++i)  // 16 positions: 8 columns of P, 2048 bytes of V
+                  umma_f16_ts(t_o, t_s + b * kWideHalf + uint32_t(i * 8), v + uint64_t(i) * 128u, idesc_o, added > first || i > 0 ? 1u : 0u);
+                if (split || half == 1) umma_commit(&kv_empty[v_at % kWideStages]);
+                ++added;
+                if (added + 1 == last || last - first == 1) umma_commit(&o_late[w]);  // once an item
+                if (added == last) umma_commit(&o_full[w]);
+                idle = 0;
               }
-              ph_p ^= 1u;
-              k = k1;
-              v = v1;
+            }
+            if ((idle & 1023u) == 1023u) {  // nothing for a while
+              const uint64_t now = globaltimer_ns();
+              if (idle == 1023u) since = now;
+              if (*abort_flag || now - since > kPagedTimeoutNs) {
+                *abort_flag = 1;
+                break;
+              }
             }
           }
-          for (; passed < n; ++passed) {
-            give_up();
-            give_up();
-          }
+          base = end;
           items.give_back_alone();
         }
         umma_commit(&mma_done);
@@ -632,7 +595,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
       }
       WideWalk walk(args, first_item, last);
-      uint32_t ph = 1;
+      uint32_t ph[2] = {1, 1};
       int sent[2] = {0, 0};
       for (;;) {
         const WideItem x = walk.next();
@@ -640,8 +603,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         const int G = args.group;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          wait(&q_free[w], ph);
-          if (w * 128 >= x.rows || __any_sync(0xffffffffu, *abort_flag)) continue;
+          if (w * 128 >= x.rows) continue;
+          wait_warp(&q_free[w], ph[w]);
+          ph[w] ^= 1u;
+          if (__any_sync(0xffffffffu, *abort_flag)) continue;
           if (args.q_boxes) {
             if (elect_one()) {
               mbar_expect_tx(&q_ready[w], kWideTileBytes);
@@ -664,7 +629,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
             if (lane == 0) mbar_arrive(&q_ready[w]);
           }
         }
-        ph ^= 1u;
       }
       const uint64_t since = globaltimer_ns();
 #pragma unroll

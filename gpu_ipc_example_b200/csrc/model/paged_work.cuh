@@ -184,6 +184,11 @@ struct QueueEnd {
   __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
     if (!mbar_try_wait(bar, parity) && !*abort_flag) mbar_wait(bar, parity, abort_flag, kPagedTimeoutNs);
   }
+  // The same by all lanes of a warp, which leave it together: what follows may be instructions of the whole warp.
+  __device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity) {
+    wait(bar, parity);
+    __syncwarp();
+  }
   __device__ __forceinline__ void step() {
     if (++at == kPagedQueue) {
       at = 0;
@@ -192,7 +197,7 @@ struct QueueEnd {
   }
   // nullptr behind the last item
   __device__ __forceinline__ const Item* take() {
-    wait(&q.full[at], ph);
+    wait_warp(&q.full[at], ph);
     const Item* x = &q.items[at];
     return x->valid && !__any_sync(0xffffffffu, *abort_flag) ? x : nullptr;
   }
@@ -213,7 +218,7 @@ struct QueueEnd {
   }
   // false when nothing more is wanted
   __device__ __forceinline__ bool put(const Item& x) {
-    wait(&q.empty[at], ph ^ 1u);
+    wait_warp(&q.empty[at], ph ^ 1u);
     if ((threadIdx.x & 31) == 0) {
       q.items[at] = x;
       mbar_arrive(&q.full[at]);

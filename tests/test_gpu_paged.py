@@ -167,7 +167,10 @@ def workspace(hq, hkv, max_new):
 def attend(p, hq, hkv, max_new=None, ws=None):
     q, k, v, table, total, cu = p
     max_new = max_new or max(1, max(b - a for a, b in zip(cu, cu[1:])))
-    return ops().paged_attention(q, k, v, ints(table), ints(total), ints(cu), workspace(hq, hkv, max_new) if ws is None else ws, hq, hkv, max_new)
+    ws = workspace(hq, hkv, max_new) if ws is None else ws
+    out = ops().paged_attention(q, k, v, ints(table), ints(total), ints(cu), ws, hq, hkv, max_new)
+    assert int(ws[:4].view(torch.int32)) == 0  # no wait gave up
+    return out
 
 
 def assert_attention(out, p, hq, hkv):
@@ -260,6 +263,22 @@ def test_attention_gives_the_same_bits_again():
         p = paged_problem(torch.float16, 64, hq, hkv, [3000, 10, 2000], new)
         first = attend(p, hq, hkv)
         assert all(torch.equal(first, attend(p, hq, hkv)) for _ in range(5))
+
+
+def test_attention_call_behind_call():
+    """Calls of all sorts without a pause, a workspace for all of them: every one its own result, no wait that gives up."""
+    sorts = [(8, 1, 64, [700, 20, 3000], [5, 3, 8]), (16, 2, 32, [0, 900], [20, 9]), (8, 2, 64, [1000, 0, 5], [129, 200, 1]), (8, 1, 16, [400] * 5, [1] * 5),
+             (32, 8, 128, [100, 0, 2000], [1, 700, 1]), (16, 2, 32, [3000] * 20, [5] * 20)]
+    problems = [paged_problem(torch.bfloat16, page, hq, hkv, have, new) for hq, hkv, page, have, new in sorts]
+    ws = torch.cat([workspace(8, 1, 700)])
+    args = [(q, k, v, ints(t), ints(n), ints(cu), ws, hq, hkv, max(new)) for (q, k, v, t, n, cu), (hq, hkv, _, _, new) in zip(problems, sorts)]
+    outs = [None] * len(sorts)
+    for rep in range(60):
+        for i, a in enumerate(args):
+            outs[i] = ops().paged_attention(*a)
+        assert int(ws[:4].view(torch.int32)) == 0
+    for out, p, (hq, hkv, *_) in zip(outs, problems, sorts):
+        assert_attention(out, p, hq, hkv)
 
 
 def test_attention_of_bad_pages_leaves_the_others_alone():
