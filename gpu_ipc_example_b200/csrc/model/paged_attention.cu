@@ -95,7 +95,7 @@ void paged_attention(DType t, const void* q, int64_t row_stride, const void* kca
   a.hq = s.hq;
   a.hkv = s.hkv;
   a.group = s.hq / s.hkv;
-  a.page = s.page;
+  while ((1 << a.page_log) < s.page) ++a.page_log;
   a.width = s.width;
   a.pages = s.pages;
   a.scale_log2 = 1.4426950408889634f / sqrtf(float(kAttnD));

@@ -35,13 +35,11 @@ struct NarrowCut {
   const PagedArgs& a;
   __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0 && r.n * a.group <= a.narrow_rows; }
   __device__ __forceinline__ int tiles(const Request& r) const { return (r.len + kNarTile - 1) / kNarTile; }
-  __device__ __forceinline__ int64_t length(const Request& r) const { return takes(r) ? int64_t(a.hkv) * (kNarStart + tiles(r)) : 0; }
-  __device__ __forceinline__ Start place(const Mark& m) const {
-    if (m.request >= a.requests) return Start{a.requests, 0, 0, 0, 0, 0, 0};
-    const Request r = request_at(a, m.request);
-    const int per = kNarStart + tiles(r);
-    const int h = int(divide(m.offset, per));
-    return Start{m.request, h, max(0, int(m.offset - int64_t(h) * per) - kNarStart), r.n * a.group, int64_t(r.row0) * a.hq + h * a.group, 0, 0};
+  __device__ __forceinline__ uint64_t length(const Request& r) const { return takes(r) ? uint64_t(a.hkv) * uint32_t(kNarStart + tiles(r)) : 0; }
+  __device__ __forceinline__ Start place(const Request& r, int request, uint64_t offset) const {
+    const uint32_t per = uint32_t(kNarStart + tiles(r));
+    const int h = int(divide(offset, per));
+    return Start{request, h, max(0, int(offset - uint64_t(h) * per) - kNarStart), h, 0, r.n * a.group, r};
   }
 };
 
@@ -60,6 +58,8 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   __shared__ Items s_queue;
   __shared__ uint64_t full[kNarStages], empty[kNarStages];
   __shared__ int s_abort;
+  __shared__ uint64_t s_sum[kNarThreads / 32];
+  __shared__ Start s_span[2];
   __shared__ float2 s_ml[kNarWarps][8];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_o = reinterpret_cast<float*>(ring + kNarStages * 2 * kNarTileBytes);  // [8 warps][8 rows][kNarORow]
@@ -78,56 +78,55 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   pdl_wait();
   reset_status(args);
   const NarrowCut cut{args};
-  Mark marks[2];
-  find_span<kNarThreads>(args, [&](const Request& r) { return cut.length(r); }, kNarLeast, warp == kNarWarps + 1, reinterpret_cast<int64_t*>(ring), marks);
+  find_span<kNarThreads>(
+      args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); }, kNarLeast, s_sum, s_span);
+  __syncthreads();
   QueueEnd<Items, NarrowItem> items{s_queue, abort_flag};
 
   if (warp == kNarWarps + 1) {
     // ---- the walk ------------------------------------------------------------------------------------------------------------
-    const Start first = cut.place(marks[0]), last = cut.place(marks[1]);
+    const Start first = s_span[0], last = s_span[1];
     if (lane == 0) {
       args.starts[blockIdx.x] = first;
       if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
     }
-    const auto takes = [&](const Request& r) { return cut.takes(r); };
     Window win;
-    int i = first.request < args.requests ? win.next(args, first.request, takes) : args.requests, h = first.number, t0 = first.tile;
-    for (bool more = true; more;) {
+    Request r = first.r;
+    int i = first.request, h = first.number, t0 = first.tile;
+    for (;;) {
       NarrowItem x{};
       if (i < args.requests && !(i > last.request || (i == last.request && (h > last.number || (h == last.number && t0 >= last.tile))))) {
-        const Request r = win.get(i);
         const int tiles = cut.tiles(r), t1 = i == last.request && h == last.number ? last.tile : tiles;
         x = NarrowItem{1, i, h, r.row0, r.n, r.len, t0, t1, t0 == 0 && t1 == tiles};
-        t0 = 0;
-        if (++h == args.hkv) {
-          h = 0;
-          i = win.next(args, i + 1, takes);
-        }
       }
-      more = items.put(x);
+      if (!items.put(x)) break;
+      t0 = 0;
+      if (++h == args.hkv) {
+        h = 0;
+        i = win.next(args, i + 1, [&](const Request& y) { return cut.takes(y); });
+        if (i < args.requests) r = win.get(i);
+      }
     }
   } else if (warp == kNarWarps) {
     // ---- the stream: lane l knows where box l of a tile is; K and V, left and right half of the dimensions --------------------
-    const int box = min(args.page, kNarTile), boxes = kNarTile / box, per_page = args.page / box;
-    const int outside = int(args.pages * args.hkv * args.page);
+    const int box_log = min(args.page_log, 6), box = 1 << box_log, boxes_log = 6 - box_log, boxes = 1 << boxes_log, per_page = args.page_log - box_log;
     uint32_t st = 0, ph = 0;
     int issued = 0;
     for (const NarrowItem* x = items.take(); x != nullptr; x = items.take()) {
       const int* table = args.table + int64_t(x->request) * args.width;
-      const int len = x->len, h = x->h, t1 = x->t1, pages = (len + args.page - 1) / args.page;
+      const int len = x->len, h = x->h, t1 = x->t1, pages = (len + (1 << args.page_log) - 1) >> args.page_log;
       int base = -64, entry = 0;  // 32 entries of the request's table, one per lane
       for (int t = x->t0; t < t1; ++t) {
-        const int b = t * boxes + (lane & (boxes - 1)), p = b / per_page;
-        if ((t * boxes + boxes - 1) / per_page >= base + 32) {
-          base = t * boxes / per_page;
+        const int b0 = t << boxes_log;
+        if (((b0 + boxes - 1) >> per_page) >= base + 32) {
+          base = b0 >> per_page;
           entry = base + lane < pages ? table[base + lane] : -1;
         }
-        const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
-        const int at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
-        const int n = min(boxes, (len - t * kNarTile + box - 1) / box);  // boxes that hold positions of the request
+        const int at = box_row(args, h, b0 + (lane & (boxes - 1)), box_log, entry, base);
+        const int n = min(boxes, (len - t * kNarTile + box - 1) >> box_log);  // boxes that hold positions of the request
         items.wait_warp(&empty[st], ph ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
-        if (lane == 0) mbar_expect_tx(&full[st], uint32_t(n * box) * kAttnD * 4u);
+        if (lane == 0) mbar_expect_tx(&full[st], uint32_t(n << box_log) * kAttnD * 4u);
         __syncwarp();
         unsigned char* dst = ring + st * 2 * kNarTileBytes;
         for (int k = 0; k < n; ++k, dst += box * 128) {

@@ -62,35 +62,36 @@ struct WideCut {
   }
   __device__ __forceinline__ int tiles(const Request& r, int item) const { return (seen(r, (item + 1) * kWideRows) + kWideTile - 1) / kWideTile; }
   // Length of the first `t` items of a head, in positions x group: item u sees max(len - n, 0) + (u + 1) * 256 / group positions or a few less.
-  __device__ __forceinline__ int64_t before(const Request& r, int64_t t) const {
-    return t * (int64_t(max(0, r.len - r.n)) + kWideStart) * a.group + (kWideRows / 2) * t * (t + 1);
+  __device__ __forceinline__ uint64_t before(const Request& r, uint32_t t) const {
+    return uint64_t(t) * (uint32_t(max(0, r.len - r.n) + kWideStart) * uint64_t(a.group) + (kWideRows / 2) * (t + 1));
   }
-  __device__ __forceinline__ int64_t length(const Request& r) const { return takes(r) ? a.hkv * before(r, items(r)) : 0; }
+  __device__ __forceinline__ uint64_t length(const Request& r) const { return takes(r) ? uint32_t(a.hkv) * before(r, uint32_t(items(r))) : 0; }
   __device__ __forceinline__ Start start(const Request& r, int request, int h, int item, int n, int tile) const {
-    return Start{request, h * n + item, tile, min(kWideRows, r.n * a.group - item * kWideRows), int64_t(r.row0) * a.hq + int64_t(h) * a.group, item * kWideRows, 0};
+    return Start{request, h * n + item, tile, h, item * kWideRows, min(kWideRows, r.n * a.group - item * kWideRows), r};
   }
-  __device__ __forceinline__ Start place(const Mark& m) const {
-    if (m.request >= a.requests) return Start{a.requests, 0, 0, 0, 0, 0, 0};
-    const Request r = request_at(a, m.request);
+  __device__ __forceinline__ Start place(const Request& r, int request, uint64_t offset) const {
     const int n = items(r);
-    const int64_t per = before(r, n);
-    const int h = int(divide(m.offset, per));
-    const int64_t rest = m.offset - h * per;
-    int lo = 0, hi = n;  // the last item that begins at or before `rest`
+    const uint64_t per = before(r, uint32_t(n));
+    int h = 0;
+    while (offset >= per) {  // a few heads
+      offset -= per;
+      ++h;
+    }
+    int lo = 0, hi = n;  // the last item that begins at or before it
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (before(r, mid) <= rest) lo = mid;
+      if (before(r, uint32_t(mid)) <= offset) lo = mid;
       else hi = mid;
     }
-    const int64_t in = rest - before(r, lo) - int64_t(kWideStart) * a.group;
-    const int t = in <= 0 ? 0 : int(divide(in + int64_t(kWideTile / 2) * a.group, int64_t(kWideTile) * a.group));
+    const uint64_t in = offset - before(r, uint32_t(lo)), skip = uint64_t(kWideStart) * uint32_t(a.group);
+    const int t = in <= skip ? 0 : int(divide(in - skip + uint64_t(kWideTile / 2) * uint32_t(a.group), uint32_t(kWideTile * a.group)));
     const int all = tiles(r, lo);
     if (t >= all && all > 0) {  // rounded to its end: the next item
-      if (lo + 1 < n) return start(r, m.request, h, lo + 1, n, 0);
-      if (h + 1 < a.hkv) return start(r, m.request, h + 1, 0, n, 0);
-      return Start{m.request + 1, 0, 0, 0, 0, 0, 0};
+      if (lo + 1 < n) return start(r, request, h, lo + 1, n, 0);
+      if (h + 1 < a.hkv) return start(r, request, h + 1, 0, n, 0);
+      return Start{request + 1};
     }
-    return start(r, m.request, h, lo, n, min(t, max(all - 1, 0)));
+    return start(r, request, h, lo, n, min(t, max(all - 1, 0)));
   }
 };
 
@@ -225,6 +226,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   __shared__ float2 s_ml[128];  // maxima and sums of w = 1
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ uint64_t s_sum[kWideThreads / 32];
+  __shared__ Start s_span[2];
   unsigned char* q_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = q_smem + 2 * kWideTileBytes;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = int(threadIdx.x & 31);
@@ -259,8 +262,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   pdl_wait();
   reset_status(args);
   const WideCut cut{args};
-  Mark marks[2];
-  find_span<kWideThreads>(args, [&](const Request& r) { return cut.length(r); }, int64_t(kWideLeast) * args.group, warp == 11, reinterpret_cast<int64_t*>(ring), marks);
+  find_span<kWideThreads>(
+      args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); },
+      uint32_t(kWideLeast * args.group), s_sum, s_span);
+  __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
   QueueEnd<Items, WideItem> items{s_queue, abort_flag};
@@ -455,14 +460,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   } else {
     if (warp == 8) {
       // ---- the stream: K and V of a tile after the other.  Lane l knows where box l of it is. -------------------------------
-      const int box = min(args.page, 64), boxes = kWideTile / box, per_page = args.page / box;
-      const int outside = int(args.pages * args.hkv * args.page);
+      const int box_log = min(args.page_log, 6), box = 1 << box_log, boxes_log = 7 - box_log, boxes = 1 << boxes_log, per_page = args.page_log - box_log;
       uint32_t st = 0, ph = 0;
       int issued = 0;
       auto load = [&](const CUtensorMap* map, int at, int n) {
         wait_warp(&kv_empty[st], ph ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) return;
-        if (lane == 0) mbar_expect_tx(&kv_full[st], uint32_t(n * box) * kAttnD * 2u);
+        if (lane == 0) mbar_expect_tx(&kv_full[st], uint32_t(n << box_log) * kAttnD * 2u);
         __syncwarp();
         unsigned char* dst = ring + st * kWideTileBytes;
         for (int k = 0; k < n; ++k, dst += box * 128) {
@@ -481,17 +485,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       };
       for (const WideItem* x = items.take(); x != nullptr; x = items.take()) {
         const int* table = args.table + int64_t(x->request) * args.width;
-        const int len = x->len, h = x->h, t1 = x->t1, pages = (len + args.page - 1) / args.page;
+        const int len = x->len, h = x->h, t1 = x->t1, pages = (len + (1 << args.page_log) - 1) >> args.page_log;
         int base = -64, entry = 0;  // 32 entries of the request's table, one per lane
         for (int t = x->t0; t < t1; ++t) {
-          const int b = t * boxes + (lane & (boxes - 1)), p = b / per_page;
-          if ((t * boxes + boxes - 1) / per_page >= base + 32) {
-            base = t * boxes / per_page;
+          const int b0 = t << boxes_log;
+          if (((b0 + boxes - 1) >> per_page) >= base + 32) {
+            base = b0 >> per_page;
             entry = base + lane < pages ? table[base + lane] : -1;
           }
-          const int64_t id = __shfl_sync(0xffffffffu, entry, p - base);
-          const int at = id >= 0 && id < args.pages ? int((id * args.hkv + h) * args.page + (b - p * per_page) * box) : outside;
-          const int n = min(boxes, (len - t * kWideTile + box - 1) / box);  // boxes that hold positions of the request
+          const int at = box_row(args, h, b0 + (lane & (boxes - 1)), box_log, entry, base);
+          const int n = min(boxes, (len - t * kWideTile + box - 1) >> box_log);  // boxes that hold positions of the request
           load(&args.tma_k, at, n);
           load(&args.tma_v, at, n);
         }
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       __syncwarp();
     } else {
       // ---- the walk, and Q: by TMA where a tile of 128 rows is whole tokens, else 16 lanes a row, one 16-byte chunk each -----------
-      const Start first_item = cut.place(marks[0]), last = cut.place(marks[1]);
+      const Start first_item = s_span[0], last = s_span[1];
       if (lane == 0) {
         args.starts[blockIdx.x] = first_item;
         if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;

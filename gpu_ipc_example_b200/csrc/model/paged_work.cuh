@@ -21,14 +21,16 @@ namespace b200ipc {
 constexpr uint64_t kPagedTimeoutNs = 2000000000;  // a wait inside a CTA takes microseconds
 constexpr int kPagedQueue = 4;                    // items handed out ahead
 
-// Where a span starts: on tile `tile` of an item, and what the join has to know of that item.
+struct Request {
+  int row0, n, len;  // first row of q, new tokens, tokens in the cache
+};
+
+// Where a span starts: on tile `tile` of an item, and what the walking warp and the join have to know of that.
 struct Start {
   int request, number, tile;  // number: of the request's items, KV head by KV head
-  int rows;                   // of the item
-  int64_t out_row0;           // (first row of q) x hq + first head: a request's row r is out row out_row0 + r / group x hq + r % group
-  int row0, pad;              // its first row within the request
+  int h, row0, rows;          // of the item: KV head, first row within the request, rows
+  Request r;
 };
-static_assert(sizeof(Start) == 32);
 
 struct PagedArgs {
   alignas(64) CUtensorMap tma_k, tma_v;  // [pages * hkv * page, 128], boxes of 64 columns x min(page, 64) rows
@@ -41,7 +43,7 @@ struct PagedArgs {
   int* status;      // 0, or 1 when a wait gave up
   int64_t row_stride;
   int rows, requests, hq, hkv, group;
-  int page, width;
+  int page_log, width;  // positions of a page: a power of two
   int64_t pages;
   int narrow_rows;  // items of up to so many rows belong to the narrow kernel, the others to the wide one
   int q_boxes;      // whether tma_q is there: 128 is a multiple of the group
@@ -56,15 +58,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-struct Request {
-  int row0, n, len;  // first row of q, new tokens, tokens in the cache
-};
 __device__ __forceinline__ Request request_at(const PagedArgs& a, int i) {
   Request r;
   const int from = a.cu_new[i], to = a.cu_new[i + 1], len = a.lens[i];
   r.row0 = min(max(from, 0), a.rows);
   r.n = min(max(to, r.row0), a.rows) - r.row0;
-  r.len = min(max(len, 0), a.width * a.page);
+  r.len = min(max(len, 0), a.width << a.page_log);
   return r;
 }
 
@@ -93,74 +92,61 @@ struct Window {
   }
 };
 
-struct Mark {
-  int request;
-  int64_t offset;  // on the request's own part of the axis
-};
-// Start and end of this CTA's span.  All threads of the block take part, the marks are the walking warp's (`walks`).  `length` of a request:
-// its part of the axis, 0 for one that is not this kernel's.  No span is shorter than `least` but where the axis ends.  s_sum: THREADS words of
-// the ring, which nothing is copied to yet.
-// Divisions of 64-bit integers cost 300 clocks each here, ten of them 1.5 us of a call of ten; so quotients are fp64 products, which round
-// alike in all CTAs and grow with the span's number: all that the cuts need.
-template <int THREADS, typename Length>
-__device__ __forceinline__ void find_span(const PagedArgs& a, Length length, int64_t least, bool walks, int64_t* s_sum, Mark (&marks)[2]) {
-  __shared__ Mark s_marks[2];
-  constexpr int kPer = THREADS / 32;
-  const int each = (a.requests + THREADS - 1) / THREADS;
+// x / y, where x mostly fits 32 bits
+__device__ __forceinline__ uint64_t divide(uint64_t x, uint32_t y) {
+  return (x >> 32) == 0 ? uint64_t(uint32_t(x) / y) : x / y;
+}
+// Where this CTA's span starts and ends, into s_span.  All threads of the block; a barrier has to follow.  `length` of a request: its part of
+// the axis, 0 for one that is not this kernel's; `place`: where on it an offset is.  No span is shorter than `least` but where the axis ends.
+// Code that runs once runs at the speed at which it is fetched (20 clocks an instruction and more), so there is as little of it as
+// can be, the same for all warps, and no division of 64 bits (300 clocks) unless the axis is that long.  s_sum: THREADS / 32 words.
+template <int THREADS, typename Length, typename Place>
+__device__ __forceinline__ void find_span(const PagedArgs& a, Length length, Place place, uint32_t least, uint64_t* s_sum, Start* s_span) {
+  const int lane = int(threadIdx.x & 31), warp = int(threadIdx.x >> 5);
+  const int each = (a.requests + THREADS - 1) / THREADS;  // one, mostly
   const int i0 = min(a.requests, int(threadIdx.x) * each), i1 = min(a.requests, i0 + each);
-  int64_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine += length(request_at(a, i));
-  s_sum[threadIdx.x] = mine;
-  __syncthreads();
-  if (!walks) return;
-  const int lane = int(threadIdx.x & 31);
-  if (lane < 2) s_marks[lane] = {a.requests, 0};
-  int64_t v[kPer], sum = 0;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) sum += v[j] = s_sum[lane * kPer + j];
-  int64_t in = sum;
-#pragma unroll
+  Request r{0, 0, 0};
+  uint64_t mine = 0;
+  for (int i = i0; i < i1; ++i) {
+    r = request_at(a, i);
+    mine += length(r);
+  }
+  uint64_t in = mine;
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, in, o);
+    const uint64_t x = __shfl_up_sync(0xffffffffu, in, o);
     if (lane >= o) in += x;
   }
-  const int64_t total = __shfl_sync(0xffffffffu, in, 31);
-  const double spans = fmin(double(gridDim.x), fmax(1.0, floor(double(total) * (1.0 / double(least)))));
-  const double per_span = double(total) / spans;
-  __syncwarp();
+  if (lane == 31) s_sum[warp] = in;
+  if (threadIdx.x < 2) s_span[threadIdx.x] = Start{a.requests};
+  __syncthreads();
+  uint64_t before = in - mine, total = 0;
 #pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  const uint32_t spans = uint32_t(min(uint64_t(gridDim.x), max(uint64_t(1), divide(total, least))));
+  const uint64_t per = divide(total, spans);
+  const uint32_t more = uint32_t(total - per * spans);  // the first so many spans are longer by one
+#pragma unroll 1
   for (int k = 0; k < 2; ++k) {
-    const int c = int(blockIdx.x) + k;
-    const int64_t at = double(c) >= spans ? total : min(total, int64_t(per_span * double(c)));
-    int64_t before = in - sum;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (at >= before && at < before + v[j]) {
-        int64_t o = at - before;
-        const int t = lane * kPer + j;
-        for (int i = t * each; i < min(a.requests, (t + 1) * each); ++i) {
-          const int64_t len = each == 1 ? v[j] : length(request_at(a, i));
-          if (o < len) {
-            s_marks[k] = {i, o};
-            break;
-          }
-          o -= len;
+    const uint32_t c = blockIdx.x + uint32_t(k);
+    const uint64_t at = c < spans ? per * c + min(c, more) : total;
+    if (at >= before && at < before + mine) {
+      uint64_t o = at - before;
+      int i = i0;
+      if (each > 1) {
+        for (;; ++i) {
+          r = request_at(a, i);
+          const uint64_t l = length(r);
+          if (o < l) break;
+          o -= l;
         }
       }
-      before += v[j];
+      s_span[k] = place(r, i, o);
     }
   }
-  __syncwarp();
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // copies may go there now
-  marks[0] = s_marks[0];
-  marks[1] = s_marks[1];
-}
-// floor(x / y) of whole numbers below 2^53, by a product with the quotient put right
-__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
-  int64_t q = int64_t(double(x) / double(y));
-  if (q * y > x) --q;
-  else if (x - q * y >= y) ++q;
-  return q;
 }
 
 // The queue: the walking warp fills a place, READERS warps give it back.
@@ -175,6 +161,14 @@ struct Queue {
     }
   }
 };
+// The box of a cache's tensor map that is box `b` of a request's tiles (boxes of 1 << box_log positions), one lane each: `entry` holds 32
+// entries of its table from `base` on.  A page that the cache does not have is a box outside of it.
+__device__ __forceinline__ int box_row(const PagedArgs& a, int h, int b, int box_log, int entry, int base) {
+  const int page = b >> (a.page_log - box_log);
+  const int64_t id = __shfl_sync(0xffffffffu, entry, page - base);
+  const int64_t at = id >= 0 && id < a.pages ? (id * a.hkv + h) << a.page_log : (a.pages * a.hkv) << a.page_log;
+  return int(at) + (id >= 0 && id < a.pages ? (b << box_log) & ((1 << a.page_log) - 1) : 0);
+}
 // One warp's place in it.
 template <typename Q, typename Item>
 struct QueueEnd {
@@ -276,19 +270,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int c = int(blockIdx.x), warp = int(threadIdx.x >> 5), lane = int(threadIdx.x & 31);
   const Start here = a.starts[c], next = a.starts[c + 1];
   int k = c + 2 + int(threadIdx.x);  // where the spans behind start
-  Start from = k <= spans ? a.starts[k] : Start{-1, 0, 0, 0, 0, 0, 0};
+  Start from = k <= spans ? a.starts[k] : Start{-1};
   const int row0 = int(blockIdx.y) * kJoinRows;
   if (next.tile == 0 || (here.request == next.request && here.number == next.number && here.tile > 0) || row0 >= next.rows) return;
   int pieces = 2;  // one in this span, and in each of the following ones that start inside of the item
   for (int base = c + 2; base <= spans; base += kJoinThreads) {
     pieces += __syncthreads_count(from.request == next.request && from.number == next.number && from.tile > 0);
     k += kJoinThreads;
-    from = k <= spans ? a.starts[k] : Start{-1, 0, 0, 0, 0, 0, 0};
+    from = k <= spans ? a.starts[k] : Start{-1};
   }
   auto write = [&](const Joined& x, int row) {
     const float inv = x.l == 0 ? 0.f : 1 / x.l;
     const int at = next.row0 + row, j = at / a.group;
-    T* dst = static_cast<T*>(a.out) + (next.out_row0 + int64_t(j) * a.hq + (at - j * a.group)) * kAttnD + lane * 4;
+    T* dst = static_cast<T*>(a.out) + (int64_t(next.r.row0 + j) * a.hq + int64_t(next.h) * a.group + (at - j * a.group)) * kAttnD + lane * 4;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x.o.x * inv, x.o.y * inv), pack2<T>(x.o.z * inv, x.o.w * inv));
   };
   auto gather = [&](int row, int first, int step) {
