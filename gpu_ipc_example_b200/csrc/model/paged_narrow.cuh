@@ -2,7 +2,8 @@
 // decoding server, a few drafts behind them.
 //
 // Bound by memory: every position of a request is 512 bytes of K and V per KV head and read once for all of the item's rows.  One warp
-// streams the pages by TMA (128-byte swizzle) into a ring of six stages of 64 positions, 192 KB in flight per SM; a page that the cache
+// streams the pages by TMA (128-byte swizzle) into a ring of four stages of 64 positions, 128 KB in flight per SM (six
+// are no faster, and leave no room for the next kernel's CTAs to come up); a page that the cache
 // does not have is a box outside of the tensor, which reads zeros.  Eight warps compute with mma.sync (m16n8k16): 16 rows cannot fill
 // tcgen05's 128.  Warps 0-3 take the tiles in even stages, 4-7 those in odd ones (always the same stages: a wait for a stage's next round
 // must come from who has seen the round before, as copies may land out of order), 16 positions of a tile each.  Scores, maxima, sums
@@ -15,14 +16,14 @@ namespace b200ipc {
 
 constexpr int kNarRows = 16;
 constexpr int kNarTile = 64;     // positions
-constexpr int kNarStages = 6;    // even: a stage belongs to one half of the warps
+constexpr int kNarStages = 4;    // even: a stage belongs to one half of the warps
 constexpr int kNarWarps = 8;     // that compute; then the stream's and the walking one
 constexpr int kNarThreads = (kNarWarps + 2) * 32;
 constexpr int kNarTileBytes = kNarTile * kAttnD * 2;  // of K or V
 constexpr int kNarORow = kAttnD + 4;                  // floats of a row of the merge buffer
 constexpr size_t kNarSmem = 1024 + size_t(kNarStages) * 2 * kNarTileBytes + size_t(kNarWarps) * 8 * kNarORow * 4;
 constexpr int kNarStart = 1;     // what an item's start and end cost, in tiles
-constexpr int kNarLeast = 2;     // a span is at least so long: more than kNarStart, so that every cut leaves a tile on both sides
+constexpr int kNarLeast = 4;     // a span is at least so long: more than kNarStart, so that every cut leaves a tile on both sides
 
 struct NarrowItem {
   int valid;
@@ -197,18 +198,18 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           const uint32_t kt = ring_addr + st * 2 * kNarTileBytes, vt = kt + kNarTileBytes;
           const int pos = t * kNarTile + at;
           if (pos < len) {
-            float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, s2[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // two chains: half as long
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               uint32_t kf[4];
               nar_ldmatrix(kf, chunk_addr(kt, k_row, 2 * k + k_chunk));
-              mma_16816<T>(s[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[0], kf[1]);
-              mma_16816<T>(s[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[2], kf[3]);
+              mma_16816<T>(k & 1 ? s2[0] : s[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[0], kf[1]);
+              mma_16816<T>(k & 1 ? s2[1] : s[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], kf[2], kf[3]);
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[j][e] *= args.scale_log2;
+              for (int e = 0; e < 4; ++e) s[j][e] = (s[j][e] + s2[j][e]) * args.scale_log2;
             if (pos + 16 > all_see) {
 #pragma unroll
               for (int j = 0; j < 2; ++j)

@@ -48,21 +48,46 @@ struct Weights {
   __device__ __forceinline__ double at(int64_t i) const { return of(p[i], q ? q[i] : 0.f, i); }
 };
 
+__device__ __forceinline__ double warp_sum(double s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+__device__ __forceinline__ double warp_prefix(double s, int lane) {  // of this lane's value and those before
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += x;
+  }
+  return s;
+}
 // Sum of the words [i0, i1) by one warp; the same order in every call.
 __device__ double run_sum(const Weights& w, int64_t i0, int64_t i1, int lane, bool vec) {
   double s = 0;
   if (vec) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = i0 + lane * 4; i < i1; i += 128) {
       const float4 x = *reinterpret_cast<const float4*>(w.p + i), y = w.q ? *reinterpret_cast<const float4*>(w.q + i) : make_float4(0, 0, 0, 0);
       s += (w.of(x.x, y.x, i) + w.of(x.y, y.y, i + 1)) + (w.of(x.z, y.z, i + 2) + w.of(x.w, y.w, i + 3));
     }
   } else {
+#pragma unroll 8
     for (int64_t i = i0 + lane; i < i1; i += 32) s += w.at(i);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
+  return warp_sum(s);
+}
+struct Found {
+  int at;         // the first place with a value whose running sum is above `goal`, else the last one with a value; -1: there is none
+  double before;  // the sum in front of it
+};
+// Among `value`s of the lanes, behind a sum of `start`.
+__device__ __forceinline__ Found find(double value, double start, double goal, int lane) {
+  const double in = warp_prefix(value, lane);
+  const unsigned some = __ballot_sync(0xffffffffu, value > 0), over = __ballot_sync(0xffffffffu, value > 0 && start + in > goal);
+  if (some == 0) return {-1, start};
+  const int at = over ? __ffs(int(over)) - 1 : 31 - __clz(int(some));
+  const double before = __shfl_sync(0xffffffffu, in - value, at);
+  return {at, start + before};
 }
 
 __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const VerifyArgs a) {
@@ -113,8 +138,9 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const Verify
     cluster_arrive();
     cluster_wait();
     double sum = 0;
-    for (int i = 0; i < kVerRuns; ++i) sum += runs[i];
-    return sum;
+#pragma unroll
+    for (int i = 0; i < kVerRuns / 32; ++i) sum += runs[lane * (kVerRuns / 32) + i];
+    return warp_sum(sum);
   };
   const double* runs = s_runs[0];
   const double first = run_sum(w, i0, i1, lane, vectors(w));
@@ -128,39 +154,40 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const Verify
     runs = s_runs[1];
   }
   const double goal = double(a.sample[r]) * total;
-  double sum = 0, before = 0;
-  int chosen = -1, last = -1;
-  for (int i = 0; i < kVerRuns; ++i) {
-    const double s = runs[i];
-    if (s > 0) last = i;
-    if (chosen < 0 && s > 0 && sum + s > goal) {
-      chosen = i;
-      before = sum;
-    }
-    sum += s;
-  }
-  if (chosen < 0) {  // rounding, or a number that is not below one: the last word with a weight
-    chosen = last;
-    before = 0;
-    for (int i = 0; i < last; ++i) before += runs[i];
+  // The run, then the lane's stretch of it, then the word.  Where no running sum is above the goal (rounding, or a number that is not below
+  // one) it is the last with a weight.
+  constexpr int kEach = kVerRuns / 32;
+  double sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += runs[lane * kEach + i];
+  const Found lanes = find(sum, 0, goal, lane);
+  int chosen = -1;
+  double before = lanes.before;
+  if (lanes.at >= 0) {
+    const Found f = find(lane < kEach ? runs[lanes.at * kEach + lane] : 0, before, goal, lane);
+    chosen = lanes.at * kEach + f.at;
+    before = f.before;
   }
   int64_t word = -1;
   if (chosen >= 0 ? run == chosen : run == 0) {
     if (chosen >= 0) {
-      double at = before;
-      int64_t some = -1;  // the last word with a weight so far
-      for (int64_t b = i0; b < i1 && word < 0; b += 32) {
-        const int64_t i = b + lane;
-        const double x = i < i1 ? w.at(i) : 0.0;
-        double in = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, in, o);
-          if (lane >= o) in += y;
-        }
+      const int64_t stretch = per / 32;
+      double mine = 0;
+#pragma unroll 8
+      for (int64_t k = 0; k < stretch; ++k) {
+        const int64_t i = i0 + lane * stretch + k;
+        if (i < i1) mine += w.at(i);
+      }
+      const Found f = find(mine, before, goal, lane);
+      double at = f.before;
+      int64_t some = -1;
+      for (int64_t k = 0; k < stretch && word < 0; k += 32) {
+        const int64_t i = i0 + f.at * stretch + k + lane;
+        const double x = k + lane < stretch && i < i1 ? w.at(i) : 0.0;
+        const double in = warp_prefix(x, lane);
         const unsigned over = __ballot_sync(0xffffffffu, x > 0 && at + in > goal), any = __ballot_sync(0xffffffffu, x > 0);
-        if (over) word = b + __ffs(int(over)) - 1;
-        if (any) some = b + 31 - __clz(int(any));
+        if (over) word = i - lane + __ffs(int(over)) - 1;
+        if (any) some = i - lane + 31 - __clz(int(any));
         at += __shfl_sync(0xffffffffu, in, 31);
       }
       if (word < 0) word = some;

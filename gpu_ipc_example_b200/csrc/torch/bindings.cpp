@@ -693,6 +693,8 @@ void check_ints(const at::Tensor& t, at::ScalarType type, at::IntArrayRef sizes,
   TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.sizes() == sizes, "b200ipc: ", op, ": ", what, " must be a contiguous ", type,
               " tensor of shape ", sizes, ", got ", t.scalar_type(), " ", t.sizes());
 }
+// Past the dispatcher: an output costs a third of a microsecond.
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt); }
 void check_one_device(std::initializer_list<const at::Tensor*> ts, const char* op) {
   const at::Device d = (*ts.begin())->device();
   for (const at::Tensor* t : ts)
@@ -728,8 +730,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_extend_op(at::T
       if (t != w) check_apart(*w, *t, op);
   }
   c10::cuda::CUDAGuard guard(table.device());
-  at::Tensor cu = at::empty({B + 1}, table.options()), slots = at::empty({rows}, table.options().dtype(at::kLong)),
-             positions = at::empty({rows}, table.options()), status = at::empty({1}, table.options());
+  at::Tensor cu = empty_on(table, {B + 1}, at::kInt), slots = empty_on(table, {rows}, at::kLong), positions = empty_on(table, {rows}, at::kInt),
+             status = empty_on(table, {1}, at::kInt);
   paged_extend(table.data_ptr<int>(), lens.data_ptr<int>(), new_lens.data_ptr<int>(), free_pages.data_ptr<int>(), n_free.data_ptr<int>(),
                cu.data_ptr<int>(), slots.data_ptr<int64_t>(), positions.data_ptr<int>(), status.data_ptr<int>(), int(B), int(table.size(1)),
                int(free_pages.numel()), int(page), int(rows), at::cuda::getCurrentCUDAStream(table.get_device()));
@@ -749,7 +751,7 @@ at::Tensor paged_trim_op(at::Tensor table, at::Tensor lens, at::Tensor keep_lens
       if (t != w) check_apart(*w, *t, op);
   }
   c10::cuda::CUDAGuard guard(table.device());
-  at::Tensor status = at::empty({1}, table.options());
+  at::Tensor status = empty_on(table, {1}, at::kInt);
   paged_trim(table.data_ptr<int>(), lens.data_ptr<int>(), keep_lens.data_ptr<int>(), free_pages.data_ptr<int>(), n_free.data_ptr<int>(),
              status.data_ptr<int>(), int(table.size(0)), int(table.size(1)), int(free_pages.numel()), int(page),
              at::cuda::getCurrentCUDAStream(table.get_device()));
@@ -781,7 +783,7 @@ at::Tensor rope_paged_append_op(at::Tensor qkv, at::Tensor kcache, at::Tensor vc
   check_one_device({&qkv, &kcache, &vcache, &slots, &positions}, op);
   check_apart(kcache, vcache, op);
   c10::cuda::CUDAGuard guard(qkv.device());
-  at::Tensor q = at::empty({qkv.size(0), hq * 128}, qkv.options());
+  at::Tensor q = empty_on(qkv, {qkv.size(0), hq * 128}, qkv.scalar_type());
   rope_paged_append(dtype_of(qkv), qkv.data_ptr(), qkv.stride(0), q.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), slots.data_ptr<int64_t>(),
                     positions.data_ptr<int>(), int(qkv.size(0)), int(hq), int(hkv), int(kcache.size(2)), kcache.size(0), theta,
                     at::cuda::getCurrentCUDAStream(qkv.get_device()));
@@ -811,7 +813,7 @@ at::Tensor paged_attention_op(at::Tensor q, at::Tensor kcache, at::Tensor vcache
               "b200ipc: paged_attention workspace too small or not 256-byte aligned");
   for (const at::Tensor* t : {&q, &kcache, &vcache, &table, &lens, &cu_new}) check_apart(workspace, *t, op);
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty({q.size(0), hq * 128}, q.options());
+  at::Tensor out = empty_on(q, {q.size(0), hq * 128}, q.scalar_type());
   if (q.size(0) == 0) return out;
   const PagedAttentionShape s{int(q.size(0)), int(table.size(0)), int(hq), int(hkv), int(page), int(table.size(1)), kcache.size(0), int(std::min(max_new, q.size(0)))};
   paged_attention(dtype_of(q), q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), table.data_ptr<int>(), lens.data_ptr<int>(),
@@ -842,7 +844,7 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts_op(at::Tensor target, const std
   if (draft) check_one_device({&target, &*draft}, op);
   if (draft_lens) check_one_device({&target, &*draft_lens}, op);
   c10::cuda::CUDAGuard guard(target.device());
-  at::Tensor out = at::empty({B, K + 1}, tokens.options()), accepted = at::empty({B}, tokens.options().dtype(at::kInt));
+  at::Tensor out = empty_on(tokens, {B, K + 1}, at::kLong), accepted = empty_on(tokens, {B}, at::kInt);
   const VerifyShape s{int(B), int(K), V, target.stride(0), target.stride(1), draft ? draft->stride(0) : 0, draft ? draft->stride(1) : 0};
   verify_drafts(target.data_ptr<float>(), draft ? draft->data_ptr<float>() : nullptr, tokens.data_ptr<int64_t>(),
                 draft_lens ? draft_lens->data_ptr<int>() : nullptr, accept.data_ptr<float>(), sample.data_ptr<float>(), out.data_ptr<int64_t>(),
