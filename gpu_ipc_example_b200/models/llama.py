@@ -23,6 +23,9 @@ takes the rest, and everything once `one_kernel` or `kernels` is set to False, `
 else or `stage_events` to a list.
 With `kernels=False` the same steps are plain PyTorch ops (the reference path of the tests).
 
+`decode` has one token for every sequence, all at one position of a cache of their own.  Requests of different lengths, prompts and
+drafts among them, share a cache in pages (`models/paged.py`): `forward_paged`, `verify`.
+
 The reference has no model code; its smoke script all-reduces decode-sized fp16 activations the way a
 tensor-parallel decoder does (script/gpu_inference_test.py:29-45).  Weights are random N(0, 0.02).
 """
@@ -271,6 +274,69 @@ class LlamaTP:
             with self._stage("down_proj_allreduce_norm"):
                 normed, h = self._reduce_norm(h, gamma_next, act, [self.wdown_run[i][l] for i in range(self.nlocal)])
         self.last_hidden = normed  # final-norm output of every local rank (replicated values)
+        self.pos += 1
+        return self.next_ids(normed)
+
+    # ------------------------------------------------------------------ requests of different lengths
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, batch, cache) -> List[torch.Tensor]:
+        """The new tokens of a step of `models/paged.py`: tokens [rows] int64, request behind request as `batch` (of `cache.extend`) has them;
+        whole prompts, chunks of them, single tokens and drafts alike.  Returns the final-norm output [rows, hidden] of every local rank.
+        Rows without a token are computed like the others and mean nothing.
+
+        A serving loop that captures steps, or that uses fusion="gemm" (whose outputs are kept by shape), takes few different
+        numbers of rows and leaves the last ones empty."""
+        cfg = self.cfg
+        if not self.kernels:
+            raise ValueError("forward_paged is for the decode kernels")
+        ops, ws = torch.ops.b200ipc, cache.workspace(batch.max_new)
+        h = [self.embed[tokens] for _ in range(self.nlocal)]
+        normed = [ops.rmsnorm(x, self.norm_attn[0], cfg.eps) for x in h]
+        for l in range(cfg.layers):
+            attn_out = []
+            for i, qkv in enumerate(self._linear(normed, [w[l] for w in self.wqkv])):
+                k, v = cache.k[i][l], cache.v[i][l]
+                q = ops.rope_paged_append(qkv, k, v, batch.slots, batch.positions, self.hq, self.hkv, cfg.rope_theta)
+                attn_out.append(ops.paged_attention(q, k, v, cache.block_table, cache.lens, batch.cu_new, ws, self.hq, self.hkv, batch.max_new))
+            normed, h = self._reduce_norm(h, self.norm_mlp[l], attn_out, [w[l] for w in self.wo_run])
+            act = [ops.silu_mul(gu) for gu in self._linear(normed, [w[l] for w in self.wgu], "gate_up")]
+            gamma_next = self.norm_attn[l + 1] if l + 1 < cfg.layers else self.norm_final
+            normed, h = self._reduce_norm(h, gamma_next, act, [w[l] for w in self.wdown_run])
+        return normed
+
+    @torch.no_grad()
+    def probabilities(self, hidden: List[torch.Tensor], temperature: float = 1.0) -> torch.Tensor:
+        """softmax(logits / temperature) over the whole vocabulary, [rows, vocab] in fp32, of hidden states of every local rank."""
+        logits = [x @ w.t() for x, w in zip(hidden, self.lm_head)]
+        if self.nlocal < self.world:
+            import torch.distributed as dist
+
+            parts = [torch.empty_like(logits[0]) for _ in range(self.world)]
+            dist.all_gather(parts, logits[0])
+            logits = parts
+        return torch.softmax(torch.cat(logits, -1).float() / temperature, -1)
+
+    @torch.no_grad()
+    def verify(self, last: torch.Tensor, drafts: torch.Tensor, draft_probs: Optional[torch.Tensor], cache, accept: torch.Tensor, sample: torch.Tensor,
+               temperature: float = 1.0):
+        """A step of speculative decoding: `last` [requests] is every request's newest token (not in the cache yet), `drafts` [requests, K] what a
+        draft model says comes next, with `draft_probs` [requests, K, vocab] (None: it is certain); accept [requests, K] and sample [requests] are
+        uniform random numbers, the same on every rank.  Returns (tokens [requests, K + 1]: the accepted drafts and one more, then -1;
+        accepted [requests]).  The cache then holds `last` and the accepted drafts; the one more is the next `last`."""
+        B, K = drafts.shape
+        before = cache.lens.clone()
+        batch = cache.extend(torch.full_like(before, K + 1), B * (K + 1), K + 1)
+        hidden = self.forward_paged(torch.cat([last[:, None], drafts], 1).view(-1), batch, cache)
+        probs = self.probabilities(hidden, temperature).view(B, K + 1, -1)
+        tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts, None, accept, sample)
+        # a step that found no room has added nothing
+        cache.trim(torch.minimum(cache.lens, before + accepted + 1))
+        return tokens, accepted
+
+    @torch.no_grad()
+    def next_ids(self, normed: List[torch.Tensor]) -> torch.Tensor:
+        """Greedy ids [rows] of final-norm outputs of every local rank."""
+        cfg = self.cfg
         # vocabulary-parallel head: local arg-max, then the global one over ranks
         best_val, best_idx = [], []
         for i in range(self.nlocal):
@@ -278,11 +344,10 @@ class LlamaTP:
             v, ix = torch.ops.b200ipc.row_argmax(logits) if self.kernels else logits.float().max(dim=-1)
             best_val.append(v)
             best_idx.append(ix + self.ranks[i] * (cfg.vocab // self.world) if self.ranks[i] else ix)
-        self.pos += 1
         if self.world == 1:
             return best_idx[0]
         if self.nlocal > 1:
-            vals = torch.stack(best_val)                       # [world, B]
+            vals = torch.stack(best_val)                       # [world, rows]
             idxs = torch.stack(best_idx)
             return idxs.gather(0, vals.argmax(0, keepdim=True))[0]
         import torch.distributed as dist
