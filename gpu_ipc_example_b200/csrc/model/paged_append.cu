@@ -97,8 +97,12 @@ void rope_paged_append(DType t, const void* qkv, int64_t row_stride, void* q_out
                        const int* positions, int rows, int hq, int hkv, int page, int64_t pages, double theta, cudaStream_t stream) {
   B200_REQUIRE(rows >= 0 && hq >= 1 && hkv >= 1 && page >= 1 && pages >= 0 && theta > 0, "rope_paged_append: bad sizes");
   if (rows == 0) return;
-  Frequencies f;
-  for (int i = 0; i < kAttnD / 2; ++i) f.inv[i] = std::pow(theta, -double(i) / (kAttnD / 2));
+  static thread_local double made_for = 0;  // 64 powers are a microsecond
+  static thread_local Frequencies f;
+  if (made_for != theta) {
+    for (int i = 0; i < kAttnD / 2; ++i) f.inv[i] = std::pow(theta, -double(i) / (kAttnD / 2));
+    made_for = theta;
+  }
   auto launch = [&](auto* type) {
     using T = std::remove_pointer_t<decltype(type)>;
     const T* x = static_cast<const T*>(qkv);

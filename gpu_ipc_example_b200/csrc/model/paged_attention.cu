@@ -34,10 +34,11 @@ CUtensorMap query_map(DType t, const PagedArgs& a) {
   return map;
 }
 
-// The workspace: a status word, then for each kernel where the spans start, then the pieces.
+// The workspace: a status word; the narrow kernel's counters and pieces; where the wide kernel's spans start, and its pieces.
 constexpr size_t kHead = 256;
 size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 size_t starts_bytes(int spans) { return round_up(size_t(spans + 1) * sizeof(Start)); }
+size_t counters_bytes(int spans) { return round_up(size_t(spans) * sizeof(unsigned int)); }
 template <int ROWS>
 size_t pieces_bytes(int spans) { return round_up(size_t(spans) * 2 * Piece<ROWS>::kFloats * sizeof(float)); }
 
@@ -53,18 +54,6 @@ void allow_smem(const void* kernel, size_t smem) {
   done.fetch_or(bit, std::memory_order_relaxed);
 }
 
-// A kernel over the spans, and the one that joins its pieces.
-template <typename T, int ROWS>
-void launch_pair(const void* kernel, int threads, size_t smem, PagedArgs& a, int spans, char* workspace, int64_t most_rows, cudaStream_t stream) {
-  a.starts = reinterpret_cast<Start*>(workspace);
-  a.part = reinterpret_cast<float*>(workspace + starts_bytes(spans));
-  allow_smem<T, ROWS>(kernel, smem);
-  void* params[] = {&a, &spans};
-  B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(unsigned(threads)), params, smem, stream, true));
-  const unsigned groups = unsigned((std::min<int64_t>(most_rows, ROWS) + kJoinRows - 1) / kJoinRows);
-  B200_CUDA_CHECK(launch_maybe_pdl(reinterpret_cast<const void*>(&paged_join_kernel<T, ROWS>), dim3(unsigned(spans), groups), dim3(kJoinThreads), params, 0, stream, true));
-}
-
 template <typename T>
 void run(PagedArgs& a, const PagedAttentionShape& s, char* workspace, int spans, cudaStream_t stream) {
   const int64_t most = int64_t(s.max_new) * a.group;  // rows of an item, or of all items of a request
@@ -73,22 +62,34 @@ void run(PagedArgs& a, const PagedAttentionShape& s, char* workspace, int spans,
   const bool wide = most > kNarRows, narrow = !wide || int64_t(s.rows) < int64_t(s.requests) * s.max_new;
   a.narrow_rows = narrow ? kNarRows : 0;
   a.leads = 1;
+  void* params[] = {&a, &spans};
   if (narrow) {
-    launch_pair<T, kNarRows>(reinterpret_cast<const void*>(&paged_narrow_kernel<T>), kNarThreads, kNarSmem, a, spans, workspace, most, stream);
-    workspace += starts_bytes(spans) + pieces_bytes<kNarRows>(spans);
+    const void* kernel = reinterpret_cast<const void*>(&paged_narrow_kernel<T>);
+    a.arrived = reinterpret_cast<unsigned int*>(workspace);
+    a.part = reinterpret_cast<float*>(workspace + counters_bytes(spans));
+    allow_smem<T, kNarRows>(kernel, kNarSmem);
+    B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(kNarThreads), params, kNarSmem, stream, true));
     a.leads = 0;
   }
   if (wide) {
+    const void* kernel = reinterpret_cast<const void*>(&paged_wide_kernel<T>);
+    workspace += counters_bytes(spans) + pieces_bytes<kNarRows>(spans);
+    a.starts = reinterpret_cast<Start*>(workspace);
+    a.part = reinterpret_cast<float*>(workspace + starts_bytes(spans));
     a.q_boxes = 128 % a.group == 0;
     if (a.q_boxes) a.tma_q = query_map(std::is_same<T, __half>::value ? DType::F16 : DType::BF16, a);
-    launch_pair<T, kWideRows>(reinterpret_cast<const void*>(&paged_wide_kernel<T>), kWideThreads, kWideSmem, a, spans, workspace, most, stream);
+    allow_smem<T, kWideRows>(kernel, kWideSmem);
+    B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(kWideThreads), params, kWideSmem, stream, true));
+    const unsigned groups = unsigned((std::min<int64_t>(most, kWideRows) + kJoinRows - 1) / kJoinRows);
+    B200_CUDA_CHECK(launch_maybe_pdl(reinterpret_cast<const void*>(&paged_join_kernel<T, kWideRows>), dim3(unsigned(spans), groups), dim3(kJoinThreads), params, 0,
+                                     stream, true));
   }
 }
 
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count) {
-  size_t n = kHead + starts_bytes(sm_count) + pieces_bytes<kNarRows>(sm_count);
+  size_t n = kHead + counters_bytes(sm_count) + pieces_bytes<kNarRows>(sm_count);
   if (int64_t(max_new) * group > kNarRows) n += starts_bytes(sm_count) + pieces_bytes<kWideRows>(sm_count);
   return n;
 }

@@ -29,7 +29,8 @@ struct NarrowItem {
   int valid;
   int request, h;       // KV head
   int first, n, len;    // the request's first row of q, its new tokens, its tokens in the cache
-  int t0, t1, whole;    // tiles of positions; whether these are all
+  int t0, t1;           // tiles of positions
+  int from, pieces;     // the span that the item begins in, and in how many it is
 };
 
 struct NarrowCut {
@@ -40,7 +41,7 @@ struct NarrowCut {
   __device__ __forceinline__ Start place(const Request& r, int request, uint64_t offset) const {
     const uint32_t per = uint32_t(kNarStart + tiles(r));
     const int h = int(divide(offset, per));
-    return Start{request, h, max(0, int(offset - uint64_t(h) * per) - kNarStart), h, 0, r.n * a.group, r};
+    return Start{request, h, max(0, int(offset - uint64_t(h) * per) - kNarStart), h, 0, r.n * a.group, r, uint64_t(h) * per};  // + the request's
   }
 };
 
@@ -61,6 +62,8 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   __shared__ int s_abort;
   __shared__ uint64_t s_sum[kNarThreads / 32];
   __shared__ Start s_span[2];
+  __shared__ Axis s_axis;
+  __shared__ int s_last;
   __shared__ float2 s_ml[kNarWarps][8];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_o = reinterpret_cast<float*>(ring + kNarStages * 2 * kNarTileBytes);  // [8 warps][8 rows][kNarORow]
@@ -80,17 +83,13 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   reset_status(args);
   const NarrowCut cut{args};
   find_span<kNarThreads>(
-      args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); }, kNarLeast, s_sum, s_span);
+      args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); }, kNarLeast, s_sum, s_span, &s_axis);
   __syncthreads();
   QueueEnd<Items, NarrowItem> items{s_queue, abort_flag};
 
   if (warp == kNarWarps + 1) {
     // ---- the walk ------------------------------------------------------------------------------------------------------------
     const Start first = s_span[0], last = s_span[1];
-    if (lane == 0) {
-      args.starts[blockIdx.x] = first;
-      if (blockIdx.x == gridDim.x - 1) args.starts[gridDim.x] = last;
-    }
     Window win;
     Request r = first.r;
     int i = first.request, h = first.number, t0 = first.tile;
@@ -98,7 +97,12 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
       NarrowItem x{};
       if (i < args.requests && !(i > last.request || (i == last.request && (h > last.number || (h == last.number && t0 >= last.tile))))) {
         const int tiles = cut.tiles(r), t1 = i == last.request && h == last.number ? last.tile : tiles;
-        x = NarrowItem{1, i, h, r.row0, r.n, r.len, t0, t1, t0 == 0 && t1 == tiles};
+        x = NarrowItem{1, i, h, r.row0, r.n, r.len, t0, t1, int(blockIdx.x), 1};
+        if (t0 > 0 || t1 < tiles) {  // its first tile may be looked for up to kNarStart behind its beginning
+          const uint64_t origin = t0 > 0 ? first.origin : last.origin;
+          x.from = span_of(s_axis, origin + kNarStart);
+          x.pieces = span_of(s_axis, origin + kNarStart + uint32_t(tiles) - 1) - x.from + 1;
+        }
       }
       if (!items.put(x)) break;
       t0 = 0;
@@ -184,7 +188,8 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
     if (x != nullptr) load_q(x);
     while (x != nullptr) {
       const int nrows = x->n * G, len = x->len, t0 = x->t0, t1 = x->t1, h = x->h, first_row = x->first;
-      const bool whole = x->whole != 0;
+      const int from = x->from, pieces = x->pieces;
+      const bool whole = pieces == 1;
       // positions that the rows see
       const int all_see = len - x->n + 1;
       const int la = r8 < nrows ? all_see + r8 / G : 0, lb = r8 + 8 < nrows ? all_see + (r8 + 8) / G : 0;
@@ -318,6 +323,29 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           }
         }
         nar_sync();
+      }
+      if (!whole) {  // who is last puts the item together
+        if (threadIdx.x == 0) {  // behind the barrier: what it releases and acquires is the other warps' as well
+          unsigned before;
+          asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(args.arrived + from) : "memory");
+          s_last = before == unsigned(pieces - 1);
+          if (s_last) args.arrived[from] = 0;  // for the next call
+        }
+        nar_sync();
+        if (s_last) {
+          for (int row = warp; row < nrows; row += kNarWarps) {
+            Joined sum;
+#pragma unroll 4
+            for (int n = 0; n < pieces; ++n) {
+              const float* p = Piece<kNarRows>::slot(args, from + n, n == 0 ? 1 : 0);
+              sum.add(__ldcg(reinterpret_cast<const float2*>(p + 2 * row)), __ldcg(reinterpret_cast<const float4*>(p + 2 * kNarRows + row * kAttnD + lane * 4)));
+            }
+            const float inv = sum.l == 0 ? 0.f : 1 / sum.l;
+            const int j = row / G;
+            T* dst = static_cast<T*>(args.out) + (int64_t(first_row + j) * args.hq + int64_t(h) * G + (row - j * G)) * kAttnD + lane * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(sum.o.x * inv, sum.o.y * inv), pack2<T>(sum.o.z * inv, sum.o.w * inv));
+          }
+        }
       }
     }
   }

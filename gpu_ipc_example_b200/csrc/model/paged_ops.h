@@ -41,7 +41,9 @@ struct PagedAttentionShape {
   int64_t pages;   // of the cache
   int max_new;     // no request has more new tokens
 };
-// out[t] = softmax(q[t] k^T / sqrt(128)) v over the positions up to and including the token's own; lens count the new tokens.
+// out[t] = softmax(q[t] k^T / sqrt(128)) v over the positions up to and including the token's own; lens count the new tokens.  The workspace is
+// zero before the first call and kept between calls, which follow one another; its first word is 0, or 1 when a wait inside a kernel
+// ran out: the result is then not valid, and the workspace has to be zeroed.
 size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count);
 void paged_attention(DType t, const void* q, int64_t row_stride, const void* kcache, const void* vcache, const int* table, const int* lens,
                      const int* cu_new, void* out, void* workspace, const PagedAttentionShape& s, int sm_count, cudaStream_t stream);

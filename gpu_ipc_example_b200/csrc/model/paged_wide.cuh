@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   __shared__ int s_abort;
   __shared__ uint64_t s_sum[kWideThreads / 32];
   __shared__ Start s_span[2];
+  __shared__ Axis s_axis;
   unsigned char* q_smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = q_smem + 2 * kWideTileBytes;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = int(threadIdx.x & 31);
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   const WideCut cut{args};
   find_span<kWideThreads>(
       args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); },
-      uint32_t(kWideLeast * args.group), s_sum, s_span);
+      uint32_t(kWideLeast * args.group), s_sum, s_span, &s_axis);
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;

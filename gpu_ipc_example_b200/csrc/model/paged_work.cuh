@@ -7,8 +7,9 @@
 // rounding everywhere.  One warp of it then walks the span and hands the items to the others through a queue in shared memory.
 //
 // An item that a cut goes through leaves pieces: fp32 sums, maxima and unscaled outputs in the workspace.  A CTA has at most two, the end
-// of an item that began in an earlier span (slot 0) and the beginning of one that goes on in the next (slot 1); the join walks them in
-// order, so the result does not depend on timing.
+// of an item that began in an earlier span (slot 0) and the beginning of one that goes on in the next (slot 1); they are joined in that
+// order, so the result does not depend on timing: by the CTA that is done last where they are small (narrow kernel), by a kernel of its own
+// where one SM would be at it for microseconds.
 #pragma once
 
 #include "../common/check.h"
@@ -30,6 +31,12 @@ struct Start {
   int request, number, tile;  // number: of the request's items, KV head by KV head
   int h, row0, rows;          // of the item: KV head, first row within the request, rows
   Request r;
+  uint64_t origin;            // where on the axis the item begins (narrow kernel)
+};
+// The axis: `spans` of `per`, the first `more` of them longer by one.
+struct Axis {
+  uint64_t per;
+  uint32_t spans, more;
 };
 
 struct PagedArgs {
@@ -38,7 +45,8 @@ struct PagedArgs {
   const void* q;
   void* out;
   const int *table, *lens, *cu_new;
-  Start* starts;    // [CTAs + 1]
+  Start* starts;    // [CTAs + 1]; wide kernel
+  unsigned int* arrived;  // [CTAs]: pieces of the item that begins in this span and goes on; zero between calls; narrow kernel
   float* part;      // [CTAs][2] pieces
   int* status;      // 0, or 1 when a wait gave up
   int64_t row_stride;
@@ -101,7 +109,7 @@ __device__ __forceinline__ uint64_t divide(uint64_t x, uint32_t y) {
 // Code that runs once runs at the speed at which it is fetched (20 clocks an instruction and more), so there is as little of it as
 // can be, the same for all warps, and no division of 64 bits (300 clocks) unless the axis is that long.  s_sum: THREADS / 32 words.
 template <int THREADS, typename Length, typename Place>
-__device__ __forceinline__ void find_span(const PagedArgs& a, Length length, Place place, uint32_t least, uint64_t* s_sum, Start* s_span) {
+__device__ __forceinline__ void find_span(const PagedArgs& a, Length length, Place place, uint32_t least, uint64_t* s_sum, Start* s_span, Axis* s_axis) {
   const int lane = int(threadIdx.x & 31), warp = int(threadIdx.x >> 5);
   const int each = (a.requests + THREADS - 1) / THREADS;  // one, mostly
   const int i0 = min(a.requests, int(threadIdx.x) * each), i1 = min(a.requests, i0 + each);
@@ -128,7 +136,8 @@ __device__ __forceinline__ void find_span(const PagedArgs& a, Length length, Pla
   }
   const uint32_t spans = uint32_t(min(uint64_t(gridDim.x), max(uint64_t(1), divide(total, least))));
   const uint64_t per = divide(total, spans);
-  const uint32_t more = uint32_t(total - per * spans);  // the first so many spans are longer by one
+  const uint32_t more = uint32_t(total - per * spans);
+  if (threadIdx.x == 0) *s_axis = Axis{per, spans, more};
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const uint32_t c = blockIdx.x + uint32_t(k);
@@ -145,8 +154,15 @@ __device__ __forceinline__ void find_span(const PagedArgs& a, Length length, Pla
         }
       }
       s_span[k] = place(r, i, o);
+      s_span[k].origin += at - o;
     }
   }
+}
+
+// The span that a place on the axis is in.
+__device__ __forceinline__ int span_of(const Axis& a, uint64_t x) {
+  const uint64_t longer = (a.per + 1) * a.more;
+  return x < longer ? int(divide(x, uint32_t(a.per + 1))) : int(a.more + divide(x - longer, uint32_t(a.per)));
 }
 
 // The queue: the walking warp fills a place, READERS warps give it back.

@@ -85,4 +85,5 @@ class PagedCache:
         if said:
             raise PagedCacheError("; ".join(text for bit, text in _REASONS.items() if said & bit))
         if self._workspace is not None and int(self._workspace[:4].view(torch.int32)):
+            self._workspace.zero_()  # counters may have been left half way
             raise PagedCacheError("a wait inside the attention ran out")
