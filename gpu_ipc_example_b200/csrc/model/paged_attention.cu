@@ -34,7 +34,7 @@ CUtensorMap query_map(DType t, const PagedArgs& a) {
   return map;
 }
 
-// The workspace: a status word; the narrow kernel's counters and pieces; where the wide kernel's spans start, and its pieces.
+// The workspace: a status word; the narrow kernel's counters, zero between calls; its pieces, or where the wide kernel's spans start and its pieces.
 constexpr size_t kHead = 256;
 size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 size_t starts_bytes(int spans) { return round_up(size_t(spans + 1) * sizeof(Start)); }
@@ -56,42 +56,37 @@ void allow_smem(const void* kernel, size_t smem) {
 
 template <typename T>
 void run(PagedArgs& a, const PagedAttentionShape& s, char* workspace, int spans, cudaStream_t stream) {
-  const int64_t most = int64_t(s.max_new) * a.group;  // rows of an item, or of all items of a request
-  // Where every request may have as many tokens as the longest, none is looked for that has few: the wide kernel takes them all (24 x 5 drafts
-  // of 16 heads on 2: 39.8 us with both kernels, 34.7 with the wide one alone).
-  const bool wide = most > kNarRows, narrow = !wide || int64_t(s.rows) < int64_t(s.requests) * s.max_new;
-  a.narrow_rows = narrow ? kNarRows : 0;
-  a.leads = 1;
   void* params[] = {&a, &spans};
-  if (narrow) {
+  // Up to 16 rows for every request: the narrow kernel.  A batch with longer ones is the wide kernel's as a whole, which for single tokens alone is
+  // behind by 6 us a call and 10 % (32 x 2048 15.1 and 20.7 us, 16 x 32768 53.2 and 60.4), but has them read while it computes for
+  // the others (a chunk of 2047 tokens among 23 requests 170 us with both kernels, 147 with this one).
+  const int64_t most = int64_t(s.max_new) * a.group;
+  if (most <= kNarRows) {
     const void* kernel = reinterpret_cast<const void*>(&paged_narrow_kernel<T>);
     a.arrived = reinterpret_cast<unsigned int*>(workspace);
     a.part = reinterpret_cast<float*>(workspace + counters_bytes(spans));
     allow_smem<T, kNarRows>(kernel, kNarSmem);
     B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(kNarThreads), params, kNarSmem, stream, true));
-    a.leads = 0;
+    return;
   }
-  if (wide) {
-    const void* kernel = reinterpret_cast<const void*>(&paged_wide_kernel<T>);
-    workspace += counters_bytes(spans) + pieces_bytes<kNarRows>(spans);
-    a.starts = reinterpret_cast<Start*>(workspace);
-    a.part = reinterpret_cast<float*>(workspace + starts_bytes(spans));
-    a.q_boxes = 128 % a.group == 0;
-    if (a.q_boxes) a.tma_q = query_map(std::is_same<T, __half>::value ? DType::F16 : DType::BF16, a);
-    allow_smem<T, kWideRows>(kernel, kWideSmem);
-    B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(kWideThreads), params, kWideSmem, stream, true));
-    const unsigned groups = unsigned((std::min<int64_t>(most, kWideRows) + kJoinRows - 1) / kJoinRows);
-    B200_CUDA_CHECK(launch_maybe_pdl(reinterpret_cast<const void*>(&paged_join_kernel<T, kWideRows>), dim3(unsigned(spans), groups), dim3(kJoinThreads), params, 0,
-                                     stream, true));
-  }
+  const void* kernel = reinterpret_cast<const void*>(&paged_wide_kernel<T>);
+  workspace += counters_bytes(spans);  // which stay zero
+  a.starts = reinterpret_cast<Start*>(workspace);
+  a.part = reinterpret_cast<float*>(workspace + starts_bytes(spans));
+  a.q_boxes = 128 % a.group == 0;
+  if (a.q_boxes) a.tma_q = query_map(std::is_same<T, __half>::value ? DType::F16 : DType::BF16, a);
+  allow_smem<T, kWideRows>(kernel, kWideSmem);
+  B200_CUDA_CHECK(launch_maybe_pdl(kernel, dim3(unsigned(spans)), dim3(kWideThreads), params, kWideSmem, stream, true));
+  const unsigned groups = unsigned((std::min<int64_t>(most, kWideRows) + kJoinRows - 1) / kJoinRows);
+  B200_CUDA_CHECK(launch_maybe_pdl(reinterpret_cast<const void*>(&paged_join_kernel<T, kWideRows>), dim3(unsigned(spans), groups), dim3(kJoinThreads), params, 0, stream,
+                                   true));
 }
 
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count) {
-  size_t n = kHead + counters_bytes(sm_count) + pieces_bytes<kNarRows>(sm_count);
-  if (int64_t(max_new) * group > kNarRows) n += starts_bytes(sm_count) + pieces_bytes<kWideRows>(sm_count);
-  return n;
+  const bool wide = int64_t(max_new) * group > kNarRows;
+  return kHead + counters_bytes(sm_count) + (wide ? starts_bytes(sm_count) + pieces_bytes<kWideRows>(sm_count) : pieces_bytes<kNarRows>(sm_count));
 }
 
 void paged_attention(DType t, const void* q, int64_t row_stride, const void* kcache, const void* vcache, const int* table, const int* lens,

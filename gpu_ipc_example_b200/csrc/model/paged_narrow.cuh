@@ -35,7 +35,7 @@ struct NarrowItem {
 
 struct NarrowCut {
   const PagedArgs& a;
-  __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0 && r.n * a.group <= a.narrow_rows; }
+  __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0 && r.n * a.group <= kNarRows; }
   __device__ __forceinline__ int tiles(const Request& r) const { return (r.len + kNarTile - 1) / kNarTile; }
   __device__ __forceinline__ uint64_t length(const Request& r) const { return takes(r) ? uint64_t(a.hkv) * uint32_t(kNarStart + tiles(r)) : 0; }
   __device__ __forceinline__ Start place(const Request& r, int request, uint64_t offset) const {

@@ -1,4 +1,5 @@
-// Attention over a paged cache for requests with more rows than the narrow kernel's: prompts, chunks of them, drafts of many heads.
+// Attention over a paged cache where a request may have more rows than the narrow kernel takes: prompts, chunks of them, drafts of many
+// heads, and whatever else is in such a batch (single tokens among chunks: their memory time passes under the chunks' arithmetic).
 //
 // Rows are (new token, query head) pairs of one KV head, a token's heads next to one another, so that a K or V tile serves all heads of
 // the group.  A CTA takes up to 256 rows over tiles of 128 positions, with two accumulators of 128 rows:
@@ -37,9 +38,13 @@ constexpr int kWideThreads = 384;  // three warpgroups
 constexpr int kWideTileBytes = kWideTile * kAttnD * 2;  // also of 128 rows of Q
 constexpr int kWideStage = 4096;  // bytes of a softmax warp's way out: 32 rows x 128
 constexpr size_t kWideSmem = 1024 + size_t(kWideStages + 2) * kWideTileBytes + 8 * kWideStage;
-constexpr int kWideStart = 192;  // what an item's start and end cost, in positions
-constexpr int kWideLeast = 384;  // a span is at least so long: more than kWideStart + a tile, so that every cut leaves a tile on both sides
+// What an item's start and end cost, in positions.  A chunk of 512 tokens at 16384: 55.0 us with 96, 52.8 with 192, 50.7 with 384, no less with more.
+constexpr int kWideStart = 384;
+constexpr int kWideLeast = 576;  // a span is at least so long: more than kWideStart + a tile, so that every cut leaves a tile on both sides
 constexpr float kWideSlack = 8.f;
+// Every so manieth pair of weights is computed on the other units: prompts of up to 4096 tokens 416 us without, 395 with every fourth, 436 with
+// every second.
+constexpr int kWidePoly = 4;
 
 // The part of an item that lies in a span.
 struct WideItem {
@@ -54,7 +59,7 @@ struct WideItem {
 
 struct WideCut {
   const PagedArgs& a;
-  __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0 && r.n * a.group > a.narrow_rows; }
+  __device__ __forceinline__ bool takes(const Request& r) const { return r.n > 0; }
   __device__ __forceinline__ int items(const Request& r) const { return (r.n * a.group + kWideRows - 1) / kWideRows; }
   // positions that the rows below `rows` of the request see
   __device__ __forceinline__ int seen(const Request& r, int rows) const {
@@ -212,6 +217,24 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
   return m;
 }
+// 2^x for two values up to 127, without the special function unit: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 whose
+// greatest relative error there is least (2.6e-6, found by Remez' exchange), n into the exponent.  From -126 down, -inf included, it is 2^-126; NaN gives what is not finite as a 16-bit weight.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
+  float2 v = f32x2_parts(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
+  x = f32x2(v.x, v.y);
+  constexpr float kWhole = 12582912.f;  // 3 x 2^22: behind the addition the last bits are n
+  const uint64_t t = f32x2_add(x, f32x2(kWhole, kWhole));
+  const uint64_t f = f32x2_fma(f32x2_add(t, f32x2(-kWhole, -kWhole)), f32x2(-1.f, -1.f), x);
+  uint64_t p = f32x2_fma(f, f32x2(0.009570102207362652f, 0.009570102207362652f), f32x2(0.05591785907745361f, 0.05591785907745361f));
+  p = f32x2_fma(p, f, f32x2(0.240247443318367f, 0.240247443318367f));
+  p = f32x2_fma(p, f, f32x2(0.6931217908859253f, 0.6931217908859253f));
+  p = f32x2_fma(p, f, f32x2(0.9999992847442627f, 0.9999992847442627f));
+  const float2 y = f32x2_parts(p), n = f32x2_parts(t);
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
+}
+
 __device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
@@ -352,8 +375,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
               uint32_t p[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                float2 y = f32x2_parts(f32x2_fma(f32x2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), f32x2(args.scale_log2, args.scale_log2), f32x2(shift, shift)));
-                y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                const uint64_t v = f32x2_fma(f32x2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), f32x2(args.scale_log2, args.scale_log2), f32x2(shift, shift));
+                float2 y;
+                if (e % kWidePoly == kWidePoly - 1) {  // what is masked gets 2^-126 here; a row with nothing else is looked after below
+                  y = exp2_poly(v);
+                } else {
+                  y = f32x2_parts(v);
+                  y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                }
                 part[e & 1] = f32x2_add(part[e & 1], f32x2(y.x, y.y));
                 p[e] = pack2<T>(y.x, y.y);
               }
@@ -372,6 +401,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       const bool split = x->split != 0, whole = x->whole != 0, both = split && x->t1 > x->t0;
       const bool busy = G0 + (warp & 3) * 32 < x->rows, exists = G0 + row < x->rows;
       const int at = x->row0 + G0 + row, j = at / G;
+      // a row that sees nothing of this accumulator's positions (it sees the first so many of the request)
+      if (!exists || x->len - x->n + j + 1 <= x->t0 * kWideTile + (split ? w * kWideHalf : 0)) {
+        ref = -INFINITY;
+        sum = 0;
+      }
       if (count > 0) {
         wait_warp(&o_full[w], ph_o);
         ph_o ^= 1u;

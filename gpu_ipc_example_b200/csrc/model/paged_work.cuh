@@ -53,9 +53,7 @@ struct PagedArgs {
   int rows, requests, hq, hkv, group;
   int page_log, width;  // positions of a page: a power of two
   int64_t pages;
-  int narrow_rows;  // items of up to so many rows belong to the narrow kernel, the others to the wide one
   int q_boxes;      // whether tma_q is there: 128 is a multiple of the group
-  int leads;        // the call's first kernel: resets the status, and writes the rows behind the last request
   float scale_log2;
 };
 
@@ -246,14 +244,13 @@ struct Piece {
   __device__ static float* slot(const PagedArgs& a, int cta, int which) { return a.part + (size_t(cta) * 2 + size_t(which)) * kFloats; }
 };
 
-// What the call's first kernel does beside its own work.  At its start: the status is good.
+// What both kernels do beside their own work.  At the start: the status is good.
 __device__ __forceinline__ void reset_status(const PagedArgs& a) {
-  if (a.leads && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
 }
-// At its end, all threads: rows behind the last request are zeros.
+// At the end, all threads: rows behind the last request are zeros.
 template <typename T>
 __device__ __forceinline__ void zero_tail(const PagedArgs& a) {
-  if (!a.leads) return;
   const int tail = min(max(a.cu_new[a.requests], 0), a.rows), vectors = a.hq * kAttnD / 8;
   for (int64_t row = int64_t(tail) + blockIdx.x; row < a.rows; row += gridDim.x)
     for (int v = int(threadIdx.x); v < vectors; v += int(blockDim.x))
