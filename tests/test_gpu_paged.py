@@ -250,11 +250,13 @@ def test_attention_of_steep_scores(dtype, new):
     assert_attention(attend(p, hq, hkv), p, hq, hkv)
 
 
-def test_attention_of_a_batch_larger_than_the_grid():
-    hq, hkv = 8, 8
-    rng = random.Random(3)
-    p = paged_problem(torch.float16, 16, hq, hkv, [rng.randint(0, 90) for _ in range(300)], [rng.randint(0, 2) for _ in range(300)])
-    assert_attention(attend(p, hq, hkv), p, hq, hkv)
+@pytest.mark.parametrize("requests,new", [(300, 2), (1000, 2), (1300, 20), (2500, 1)])
+def test_attention_of_a_batch_larger_than_the_grid(requests, new):
+    """More requests than CTAs, and than the threads that look through them."""
+    hq, hkv = 8, 4
+    rng = random.Random(requests)
+    p = paged_problem(torch.float16, 16, hq, hkv, [rng.randint(0, 60) for _ in range(requests)], [rng.choice([0, rng.randint(0, new)]) for _ in range(requests)])
+    assert_attention(attend(p, hq, hkv, max_new=new), p, hq, hkv)
 
 
 def test_attention_gives_the_same_bits_again():
@@ -337,6 +339,45 @@ def test_attention_captured_and_replayed_with_other_lengths(new, later):
         rows = p[0].shape[0]
         assert_attention(out[:rows], p, hq, hkv)
         assert (out[rows:] == 0).all()
+
+
+def test_a_cache_of_more_than_two_to_the_31_elements():
+    """Append to the last pages of caches of 4.5 GB each, and attention over them: short requests and long ones."""
+    hq, hkv, page = 8, 2, 64
+    pages = (1 << 31) // (hkv * page * D) + 2000
+    k, v = (torch.empty(pages, hkv, page, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    for new in ([1, 2], [40, 3]):
+        have = [500, 70]
+        q, ks, vs, table, total, cu = paged_problem(torch.float16, page, hq, hkv, have, new)
+        offset = pages - ks.shape[0]
+        k[offset:].copy_(ks)
+        v[offset:].copy_(vs)
+        far = [[x + offset if x >= 0 else x for x in r] for r in table]
+        out = attend((q, k, v, far, total, cu), hq, hkv)
+        assert_attention(out, (q, ks, vs, table, total, cu), hq, hkv)
+    qkv = torch.randn(3, (hq + 2 * hkv) * D, device="cuda").half()
+    slots = torch.tensor([pages * page - 1, pages * page - 777, pages * page], device="cuda")  # the last one is behind the cache
+    ops().rope_paged_append(qkv, k, v, slots, ints([0, 0, 0]), hq, hkv, 1e4)
+    x = qkv.view(3, hq + 2 * hkv, D)
+    for t, s in ((0, pages * page - 1), (1, pages * page - 777)):
+        assert torch.equal(k[s // page, :, s % page], x[t, hq:hq + hkv]) and torch.equal(v[s // page, :, s % page], x[t, hq + hkv:])
+
+
+def test_calls_on_another_stream_than_the_tensors():
+    """Each operator runs on the current stream, whichever that is."""
+    hq, hkv = 8, 2
+    stream = torch.cuda.Stream()
+    for new in ([1, 1], [60, 9]):
+        p = paged_problem(torch.bfloat16, 32, hq, hkv, [300, 77], new)
+        ws = workspace(hq, hkv, max(new))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(2_000_000)
+            q = p[0].mul(2)  # behind the pause: a call on another stream would read q before it is there
+            args = (ints(p[3]), ints(p[4]), ints(p[5]))
+            out = ops().paged_attention(q, p[1], p[2], *args, ws, hq, hkv, max(new))
+        stream.synchronize()
+        assert_attention(out, (q,) + p[1:], hq, hkv)
 
 
 # ---------------------------------------------------------------------------------------------- verification
