@@ -45,6 +45,9 @@ struct Weights {
     const double d = double(x) - double(y);
     return d > 0 && i != spare ? d : 0.0;
   }
+  __device__ __forceinline__ double of4(const float4& x, const float4& y, int64_t i) const {
+    return (of(x.x, y.x, i) + of(x.y, y.y, i + 1)) + (of(x.z, y.z, i + 2) + of(x.w, y.w, i + 3));
+  }
   __device__ __forceinline__ double at(int64_t i) const { return of(p[i], q ? q[i] : 0.f, i); }
 };
 
@@ -64,11 +67,17 @@ __device__ __forceinline__ double warp_prefix(double s, int lane) {  // of this 
 // Sum of the words [i0, i1) by one warp; the same order in every call.
 __device__ double run_sum(const Weights& w, int64_t i0, int64_t i1, int lane, bool vec) {
   double s = 0;
-  if (vec) {
-#pragma unroll 8
-    for (int64_t i = i0 + lane * 4; i < i1; i += 128) {
-      const float4 x = *reinterpret_cast<const float4*>(w.p + i), y = w.q ? *reinterpret_cast<const float4*>(w.q + i) : make_float4(0, 0, 0, 0);
-      s += (w.of(x.x, y.x, i) + w.of(x.y, y.y, i + 1)) + (w.of(x.z, y.z, i + 2) + w.of(x.w, y.w, i + 3));
+  if (vec) {  // four vectors of each row on their way at a time
+    for (int64_t b = i0 + lane * 4; b < i1; b += 512) {
+      float4 x[4], y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t i = b + k * 128;
+        x[k] = i < i1 ? *reinterpret_cast<const float4*>(w.p + i) : make_float4(0, 0, 0, 0);
+        y[k] = i < i1 && w.q ? *reinterpret_cast<const float4*>(w.q + i) : make_float4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += w.of4(x[k], y[k], b + k * 128);
     }
   } else {
 #pragma unroll 8
@@ -173,10 +182,14 @@ __global__ void __launch_bounds__(kVerThreads) verify_drafts_kernel(const Verify
     if (chosen >= 0) {
       const int64_t stretch = per / 32;
       double mine = 0;
+      const int64_t s0 = i0 + lane * stretch, s1 = min(i1, s0 + stretch);
+      if (vectors(w)) {  // a stretch is whole vectors
 #pragma unroll 8
-      for (int64_t k = 0; k < stretch; ++k) {
-        const int64_t i = i0 + lane * stretch + k;
-        if (i < i1) mine += w.at(i);
+        for (int64_t i = s0; i < s1; i += 4)
+          mine += w.of4(*reinterpret_cast<const float4*>(w.p + i), w.q ? *reinterpret_cast<const float4*>(w.q + i) : make_float4(0, 0, 0, 0), i);
+      } else {
+#pragma unroll 8
+        for (int64_t i = s0; i < s1; ++i) mine += w.at(i);
       }
       const Found f = find(mine, before, goal, lane);
       double at = f.before;
