@@ -5,6 +5,8 @@
 // of one cluster makes the same scan of all requests in its shared memory and then takes a share of the pages and tokens, whose request
 // it finds by bisection.  The lengths are written in place, so a CTA writes only when all have read (the cluster's barrier), which is
 // also why it is one cluster and not a grid.
+#include <climits>
+
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "paged_ops.h"
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(kTabThreads) paged_extend_kernel(int* table, i
       const int len = lens[i], add = new_lens[i];
       int bad = 0;
       if (len < 0 || add < 0) bad = kPagedNegative;
-      else if ((long long)(len) + add > room) bad = kPagedTooLong;
+      else if ((long long)(len) + add > min(room, (long long)(INT_MAX))) bad = kPagedTooLong;
       else v = {pages_of(len + add, page) - pages_of(len, page), add};
       if (bad) atomicOr(&s_bad, bad);
       s_len[i] = len;

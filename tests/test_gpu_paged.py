@@ -83,6 +83,15 @@ def test_extend_that_cannot_be_changes_nothing(lens, new, width, spare, rows, st
     assert (state[0].tolist(), state[1].tolist(), state[2].tolist(), int(state[3])) == before
 
 
+def test_extend_beyond_what_an_int_counts_changes_nothing():
+    """Pages so large that a row of the table holds more than 2^31 tokens."""
+    for len_, new, status in ((2 ** 31 - 2, 2, 2), (2 ** 31 - 3, 2, 0)):
+        t, l, n = ints([[0] * 2048 + [-1] * 8]), ints([len_]), ints([4])
+        cu, slots, positions, said = ops().paged_extend(t, l, ints([new]), ints([9, 8, 7, 6]), n, 1 << 20, 3)
+        assert (int(said), int(l), int(n)) == (status, len_ if status else len_ + new, 4)
+        assert positions.tolist() == ([0, 0, 0] if status else [len_, len_ + 1, 0]) and cu.tolist() == [0, 0 if status else 2]
+
+
 def test_trim_that_cannot_be_changes_nothing():
     table, free = make_table(random.Random(1), [40, 50], 4, 16, 3)
     for keep, n_free, status in (([41, 0], 3, 2), ([3, -1], 3, 8), ([0, 0], 1, 1), ([0, 0], -1, 1)):
