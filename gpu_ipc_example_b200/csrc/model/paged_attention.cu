@@ -106,6 +106,7 @@ void paged_attention(DType t, const void* q, int64_t row_stride, const void* kca
   a.hq = s.hq;
   a.hkv = s.hkv;
   a.group = s.hq / s.hkv;
+  a.max_new = s.max_new;
   while ((1 << a.page_log) < s.page) ++a.page_log;
   a.width = s.width;
   a.pages = s.pages;

@@ -80,7 +80,6 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
-  reset_status(args);
   const NarrowCut cut{args};
   find_span<kNarThreads>(
       args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); }, kNarLeast, s_sum, s_span, &s_axis);
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   }
   zero_tail<T>(args);
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) *args.status = 1;
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(args.status, kPagedGaveUp);
 }
 
 }  // namespace b200ipc

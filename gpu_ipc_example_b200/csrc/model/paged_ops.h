@@ -41,9 +41,15 @@ struct PagedAttentionShape {
   int64_t pages;   // of the cache
   int max_new;     // no request has more new tokens
 };
-// out[t] = softmax(q[t] k^T / sqrt(128)) v over the positions up to and including the token's own; lens count the new tokens.  The workspace is
-// zero before the first call and kept between calls, which follow one another; its first word is 0, or 1 when a wait inside a kernel
-// ran out: the result is then not valid, and the workspace has to be zeroed.
+// What the first word of the attention's workspace says (bits) since it was zeroed.
+constexpr int kPagedGaveUp = 1;   // a wait inside a kernel ran out: results are not valid, the workspace has to be zeroed
+constexpr int kPagedMoreNew = 2;  // a request had more new tokens than max_new: its rows may not be written
+
+// out[t] = softmax(q[t] k^T / sqrt(128)) v over the positions up to and including the token's own (0 where there are none); lens count the new
+// tokens, cu_new starts with 0, rows behind its last are zeros.  Behind a request's last position a page may hold anything, NaN included;
+// an infinity or NaN among the values of a token may reach all rows of its request (0 x inf), as in any masked product.
+// The workspace is zero before the first call and kept between calls, which follow one another; it serves calls of every shape that it is
+// large enough for.
 size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count);
 void paged_attention(DType t, const void* q, int64_t row_stride, const void* kcache, const void* vcache, const int* table, const int* lens,
                      const int* cu_new, void* out, void* workspace, const PagedAttentionShape& s, int sm_count, cudaStream_t stream);

@@ -284,7 +284,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   __syncwarp();
   tc_fence_before_sync();
   pdl_wait();
-  reset_status(args);
   const WideCut cut{args};
   find_span<kWideThreads>(
       args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); },
@@ -680,7 +679,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   __syncthreads();
   tc_fence_after_sync();
   if (warp == 9) tmem_dealloc(tmem, 512);
-  if (threadIdx.x == 0 && *abort_flag) *args.status = 1;
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(args.status, kPagedGaveUp);
 }
 
 }  // namespace b200ipc

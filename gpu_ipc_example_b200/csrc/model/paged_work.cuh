@@ -48,9 +48,9 @@ struct PagedArgs {
   Start* starts;    // [CTAs + 1]; wide kernel
   unsigned int* arrived;  // [CTAs]: pieces of the item that begins in this span and goes on; zero between calls; narrow kernel
   float* part;      // [CTAs][2] pieces
-  int* status;      // 0, or 1 when a wait gave up
+  int* status;      // what went wrong since it was zeroed (bits)
   int64_t row_stride;
-  int rows, requests, hq, hkv, group;
+  int rows, requests, hq, hkv, group, max_new;
   int page_log, width;  // positions of a page: a power of two
   int64_t pages;
   int q_boxes;      // whether tma_q is there: 128 is a multiple of the group
@@ -116,6 +116,7 @@ __device__ __forceinline__ void find_span(const PagedArgs& a, Length length, Pla
   for (int i = i0; i < i1; ++i) {
     r = request_at(a, i);
     mine += length(r);
+    if (r.n > a.max_new && blockIdx.x == 0) atomicOr(a.status, kPagedMoreNew);
   }
   uint64_t in = mine;
 #pragma unroll 1
@@ -244,11 +245,7 @@ struct Piece {
   __device__ static float* slot(const PagedArgs& a, int cta, int which) { return a.part + (size_t(cta) * 2 + size_t(which)) * kFloats; }
 };
 
-// What both kernels do beside their own work.  At the start: the status is good.
-__device__ __forceinline__ void reset_status(const PagedArgs& a) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
-}
-// At the end, all threads: rows behind the last request are zeros.
+// At the end of both kernels, all threads: rows behind the last request are zeros.
 template <typename T>
 __device__ __forceinline__ void zero_tail(const PagedArgs& a) {
   const int tail = min(max(a.cu_new[a.requests], 0), a.rows), vectors = a.hq * kAttnD / 8;

@@ -812,7 +812,8 @@ at::Tensor paged_attention_op(at::Tensor q, at::Tensor kcache, at::Tensor vcache
   check_paged_table(table, lens, page, op);
   check_ints(cu_new, at::kInt, {table.size(0) + 1}, op, "cu_new");
   TORCH_CHECK(page == 16 || page == 32 || page == 64 || page == 128, "b200ipc: paged_attention: pages of 16, 32, 64 or 128 positions, got ", page);
-  TORCH_CHECK(table.size(1) * page < (int64_t(1) << 30), "b200ipc: paged_attention: a request of 2^30 positions or more");
+  TORCH_CHECK(table.size(1) * page < (int64_t(1) << 30) && table.numel() * page < (int64_t(1) << 42) / hkv,
+              "b200ipc: paged_attention: a request of 2^30 positions or more, or 2^42 in the whole table and all heads");
   TORCH_CHECK(max_new >= 1 && max_new < (int64_t(1) << 30), "b200ipc: paged_attention: max_new must be at least 1, got ", max_new);
   TORCH_CHECK(hq / hkv <= 64, "b200ipc: paged_attention: at most 64 query heads per KV head, got ", hq / hkv);
   TORCH_CHECK(q.size(0) * (hq / hkv) < (int64_t(1) << 30), "b200ipc: paged_attention: too many rows");

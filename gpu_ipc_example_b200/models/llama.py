@@ -289,7 +289,7 @@ class LlamaTP:
         cfg = self.cfg
         if not self.kernels:
             raise ValueError("forward_paged is for the decode kernels")
-        ops, ws = torch.ops.b200ipc, cache.workspace(batch.max_new)
+        ops, ws = torch.ops.b200ipc, cache.workspace
         h = [self.embed[tokens] for _ in range(self.nlocal)]
         normed = [ops.rmsnorm(x, self.norm_attn[0], cfg.eps) for x in h]
         for l in range(cfg.layers):

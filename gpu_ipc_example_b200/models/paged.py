@@ -7,8 +7,8 @@
     cache.trim(keep_lens)                                # drafts that were turned down, requests that are done (0)
 
 Lengths, the block table and the list of free pages are on the GPU and no call here reads them back, so steps of one number of rows can be
-captured in a CUDA graph.  What a call cannot do (no pages left, a request beyond `max_len`, more tokens than rows) it leaves undone and
-says so in a word of its own; `check()`, which waits for the GPU, raises it.
+captured in a CUDA graph; all calls on one cache follow one another, on a stream or by events.  What a call cannot do (no pages left, a
+request beyond `max_len`, more tokens than rows) it leaves undone and says so in a word of its own; `check()`, which waits for the GPU, raises it.
 
 The reference has no model code and no cache.
 """
@@ -23,10 +23,11 @@ from .._ext import load
 
 _REASONS = {1: "pages run out (or do not fit the list they go back to)", 2: "a request is longer than its row of the block table, or shorter than what is to be kept",
             4: "more new tokens than rows", 8: "a negative length"}
+_ATTENTION = {1: "a wait inside the attention ran out", 2: "a request had more new tokens than max_new"}
 
 
 class PagedCacheError(RuntimeError):
-    """A step that could not be made, or a wait inside the attention that ran out."""
+    """A step that could not be made, more new tokens than were announced, or a wait inside the attention that ran out."""
 
 
 @dataclass
@@ -57,8 +58,10 @@ class PagedCache:
         self.free_pages = torch.arange(pages, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), pages, dtype=torch.int32, device=dev)
         self._said = torch.zeros(1, dtype=torch.int32, device=dev)  # all that extend and trim could not do
-        self._group, self._dev = model.hq // model.hkv, dev
-        self._workspace: Optional[torch.Tensor] = None
+        # Scratch of the attention for steps of any size: a captured step goes on using it, so it never makes room for a larger one.
+        device = dev.index if dev.index is not None else torch.cuda.current_device()
+        need = load().paged_attention_workspace_bytes(model.hq // model.hkv, max(1, min(requests * max_len, 1 << 20)), device)
+        self.workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
 
     def extend(self, new_lens: torch.Tensor, rows: int, max_new: Optional[int] = None) -> PagedBatch:
         """Room for new_lens[i] more tokens of request i ([requests] int32 on the GPU); `rows` is the size of the batch that they are the first
@@ -71,19 +74,13 @@ class PagedCache:
         """Request i keeps its first keep_lens[i] tokens; pages that are not needed for them are free again."""
         self._said.bitwise_or_(torch.ops.b200ipc.paged_trim(self.block_table, self.lens, keep_lens, self.free_pages, self.n_free, self.page))
 
-    def workspace(self, max_new: int) -> torch.Tensor:
-        """Scratch of the attention, kept; calls that use it follow one another on a stream."""
-        need = load().paged_attention_workspace_bytes(self._group, max_new, self._dev.index if self._dev.index is not None else torch.cuda.current_device())
-        if self._workspace is None or self._workspace.numel() < need:
-            self._workspace = torch.zeros(need, dtype=torch.uint8, device=self._dev)
-        return self._workspace
-
     def check(self) -> None:
         """Raises what extend, trim or the attention found wrong since the last check.  Waits for the GPU."""
-        said = int(self._said)
-        self._said.zero_()
+        said, attention = int(self._said), int(self.workspace[:4].view(torch.int32))
         if said:
-            raise PagedCacheError("; ".join(text for bit, text in _REASONS.items() if said & bit))
-        if self._workspace is not None and int(self._workspace[:4].view(torch.int32)):
-            self._workspace.zero_()  # counters may have been left half way
-            raise PagedCacheError("a wait inside the attention ran out")
+            self._said.zero_()
+        if attention:
+            self.workspace.zero_()  # counters may have been left half way
+        texts = [text for bit, text in _REASONS.items() if said & bit] + [text for bit, text in _ATTENTION.items() if attention & bit]
+        if texts:
+            raise PagedCacheError("; ".join(texts))

@@ -140,6 +140,56 @@ def test_a_captured_step_serves_every_length():
         assert cache.lens.tolist() == eager.lens.tolist() == [45, 21, 60]
 
 
+@pytest.mark.parametrize("max_new", [1, 20])  # of the kernel for few rows, and of the other
+def test_more_new_tokens_than_announced_are_said(max_new):
+    cfg = LlamaConfig.tiny128()
+    with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
+        model = LlamaTP(cfg, comm, batch=1, max_ctx=8, fusion="gemm", seed=5)
+        cache = PagedCache(model, requests=2, max_len=128, pages=12, page=32)
+        tokens = torch.arange(42, device="cuda")
+        model.forward_paged(tokens, cache.extend(ints([2, 40]), 42, max_new), cache)
+        with pytest.raises(PagedCacheError, match="more new tokens than max_new"):
+            cache.check()
+        cache.trim(ints([0, 0]))
+        got = model.forward_paged(tokens, cache.extend(ints([2, 40]), 42, 40), cache)[0].clone()
+        cache.check()
+        cache.trim(ints([0, 0]))
+        assert torch.equal(got, model.forward_paged(tokens, cache.extend(ints([2, 40]), 42), cache)[0])
+        cache.check()
+
+
+def test_a_captured_step_outlives_larger_steps():
+    """The scratch that a captured step of single tokens uses is the one that a long prompt takes later."""
+    cfg = LlamaConfig.tiny128()
+    with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
+        model = LlamaTP(cfg, comm, batch=1, max_ctx=8, fusion="allreduce", seed=5)
+        cache = PagedCache(model, requests=2, max_len=512, pages=24, page=64)
+        tokens, one = torch.tensor([3, 4], device="cuda"), ints([1, 1])
+
+        def step():
+            return model.forward_paged(tokens, cache.extend(one, 2, 1), cache)[0]
+
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                out = step()
+            where = cache.workspace.data_ptr()
+            for rep in range(2):
+                cache.trim(ints([0, 0]))
+                model.forward_paged(torch.arange(400, device="cuda") % cfg.vocab, cache.extend(ints([100, 300]), 400, 300), cache)
+                graph.replay()
+                got = out.clone()
+                cache.trim(ints([100, 300]))
+                assert torch.equal(got, step())
+            cache.check()
+            comm.check()
+            assert cache.workspace.data_ptr() == where
+        torch.cuda.synchronize()
+
+
 def test_refusals():
     cfg = LlamaConfig.tiny()
     with Communicator.virtual(1, 0, staging_bytes=64 << 20) as comm:

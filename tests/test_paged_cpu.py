@@ -76,6 +76,8 @@ CASES = [
     ("paged_attention", attention_args, dict(kcache=z(3, 1, 24, 128, dtype=H), vcache=z(3, 1, 24, 128, dtype=H)), "pages of 16"),
     ("paged_attention", attention_args, dict(block_table=z(3, 4, dtype=L)), "block table"),
     ("paged_attention", attention_args, dict(block_table=z(1, 1 << 27), lens=z(1), cu_new=z(2)), "2.30 positions"),
+    ("paged_attention", attention_args, dict(q=z(1, 8192 * 128, dtype=H), kcache=z(1, 8192, 16, 128, dtype=H), vcache=z(1, 8192, 16, 128, dtype=H),
+                                             block_table=torch.empty(8, 1 << 22, dtype=I), lens=z(8), cu_new=z(9), hq=8192, hkv=8192), "2.42 in the whole table"),
     ("paged_attention", attention_args, dict(cu_new=z(3)), "cu_new"),
     ("paged_attention", attention_args, dict(lens=z(3, dtype=L)), "lens"),
     ("paged_attention", attention_args, dict(max_new=0), "max_new"),
