@@ -55,7 +55,6 @@ __device__ __forceinline__ void nar_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void nar_ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void nar_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kNarWarps * 32) : "memory"); }
 
 template <typename T>
 __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __grid_constant__ PagedArgs args) {
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
 #pragma unroll
         for (int d = 0; d < 16; ++d) *reinterpret_cast<float2*>(mine + 8 * d + 2 * c) = make_float2(o[d][2 * half], o[d][2 * half + 1]);
         if (c == 0) s_ml[warp][r8] = half == 0 ? make_float2(ma, sa) : make_float2(mb, sb);
-        nar_sync();
+        meet<kNarWarps * 32>();
         const int row = half * 8 + warp;
         if (row < nrows) {
           float2 ml[kNarWarps];
@@ -325,7 +324,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
             *reinterpret_cast<float4*>(piece + 2 * kNarRows + row * kAttnD + lane * 4) = v;
           }
         }
-        nar_sync();
+        meet<kNarWarps * 32>();
       }
       if (!whole) {  // who is last puts the item together
         if (threadIdx.x == 0) {  // behind the barrier: what it releases and acquires is the other warps' as well
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           s_last = before == unsigned(pieces - 1);
           if (s_last) args.arrived[from] = 0;  // for the next call
         }
-        nar_sync();
+        meet<kNarWarps * 32>();
         if (s_last) {
           for (int row = warp; row < nrows; row += kNarWarps) {
             Joined sum;
@@ -350,6 +349,8 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
           }
         }
       }
+    }
+    while (!meet<kNarWarps * 32>(true)) {
     }
   }
   zero_tail<T>(args);

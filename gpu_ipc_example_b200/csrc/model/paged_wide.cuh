@@ -240,7 +240,6 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t x) {
 __device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
-__device__ __forceinline__ void wide_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // the softmax warps
 
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __grid_constant__ PagedArgs args) {
@@ -451,7 +450,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
           s_ml[row] = make_float2(ref, sum);
           tc_fence_before_sync();
         }
-        wide_sync();
+        meet<256>();
         tc_fence_after_sync();
         const float2 other = s_ml[row];
         const float m = fmaxf(ref, other.x), u = m == -INFINITY ? 0.f : m;
@@ -489,9 +488,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         }
       }
       tc_fence_before_sync();  // O may be written again once this thread's next weights are there
-      if (both) wide_sync();   // of w = 1 as well
+      if (both) meet<256>();   // of w = 1 as well
       ring_at += uint32_t(2 * (x->t1 - x->t0));
       items.give_back();
+    }
+    while (!meet<256>(true)) {
     }
   } else {
     if (warp == 8) {

@@ -238,6 +238,18 @@ struct QueueEnd {
   }
 };
 
+// A barrier of the THREADS that compute; true once all of them are leaving.  After a wait that ran out some may leave an item before others, which
+// would stand at a plain barrier for good: who leaves goes on meeting the others until they leave too.
+template <int THREADS>
+__device__ __forceinline__ bool meet(bool leaving = false) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, 1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(all)
+               : "r"(uint32_t(leaving)), "n"(THREADS)
+               : "memory");
+  return all != 0;
+}
+
 // A piece: [rows] pairs (maximum in the log2 domain, sum), then [rows][128] of the output, not divided by the sum.
 template <int ROWS>
 struct Piece {
