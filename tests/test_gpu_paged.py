@@ -292,6 +292,35 @@ def test_attention_call_behind_call():
         assert_attention(out, p, hq, hkv)
 
 
+def test_two_captured_graphs_share_a_workspace():
+    """One of single tokens and one of chunks, replayed in turn with lengths that change between the replays."""
+    hq, hkv = 8, 2
+    sorts = [([500, 900], [1, 1]), ([300, 2000], [100, 60])]
+    problems = [paged_problem(torch.bfloat16, 32, hq, hkv, have, new, seed=3) for have, new in sorts]
+    ws = workspace(hq, hkv, 100)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs, outs, lens = [], [], []
+    with torch.cuda.stream(stream):
+        for (q, k, v, table, total, cu), (_, new) in zip(problems, sorts):
+            args = [q, k, v, ints(table), ints(total), ints(cu), ws, hq, hkv, max(new)]
+            ops().paged_attention(*args)
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                outs.append(ops().paged_attention(*args))
+            lens.append(args[4])
+            outs.append(args)  # alive while the graphs are
+        for less in (0, 37, 0):
+            for g, n, (_, _, _, _, total, _) in zip(graphs, lens, problems):
+                n.copy_(ints([t - less for t in total]))
+                g.replay()
+            for out, (q, k, v, table, total, cu) in zip(outs[::2], problems):
+                p = (q, k, v, table, [t - less for t in total], cu)
+                assert_attention(out, p, hq, hkv)
+        assert int(ws[:4].view(torch.int32)) == 0
+    torch.cuda.synchronize()
+
+
 def test_attention_of_bad_pages_leaves_the_others_alone():
     """Pages that the cache does not have: those requests get something finite or not, the others what they should."""
     for new in ([1, 1, 1], [100, 100, 100]):
