@@ -47,7 +47,8 @@ constexpr int kPagedMoreNew = 2;  // a request had more new tokens than max_new:
 
 // out[t] = softmax(q[t] k^T / sqrt(128)) v over the positions up to and including the token's own (0 where there are none); lens count the new
 // tokens, cu_new starts with 0, rows behind its last are zeros.  Behind a request's last position a page may hold anything, NaN included;
-// an infinity or NaN among the values of a token may reach all rows of its request (0 x inf), as in any masked product.
+// an infinity or NaN among the values of a token may reach all rows of its request (0 x inf), as in any masked product.  Outputs are fp32
+// sums of weights of up to 2^8 times values before they are divided: values of bf16 of 2^120 / positions and more may overflow there.
 // The workspace is zero before the first call and kept between calls, which follow one another; it serves calls of every shape that it is
 // large enough for.
 size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count);

@@ -221,20 +221,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
   return m;
 }
-// 2^x for two values up to 127, without the special function unit: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 whose
-// greatest relative error there is least (2.6e-6, found by Remez' exchange), n into the exponent.  From -126 down, -inf included, it is 2^-126; NaN gives what is not finite as a 16-bit weight.
+// 2^x for two values up to 127, without the special function unit: x = n + f with |f| <= 1/2, 2^f by the polynomial 1 + f q(f) of degree 4 whose
+// greatest relative error there is least (3.6e-6, found by Remez' exchange), n into the exponent.  From -127 down, -inf included, it is zero (the bits
+// of 1 less 127 in the exponent), between -127 and -126 what is below 2^-126; NaN gives what is not finite as a 16-bit weight.
 __device__ __forceinline__ float2 exp2_poly(uint64_t x) {
   float2 v = f32x2_parts(x);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.f));
   x = f32x2(v.x, v.y);
   constexpr float kWhole = 12582912.f;  // 3 x 2^22: behind the addition the last bits are n
   const uint64_t t = f32x2_add(x, f32x2(kWhole, kWhole));
   const uint64_t f = f32x2_fma(f32x2_add(t, f32x2(-kWhole, -kWhole)), f32x2(-1.f, -1.f), x);
-  uint64_t p = f32x2_fma(f, f32x2(0.009570102207362652f, 0.009570102207362652f), f32x2(0.05591785907745361f, 0.05591785907745361f));
-  p = f32x2_fma(p, f, f32x2(0.240247443318367f, 0.240247443318367f));
-  p = f32x2_fma(p, f, f32x2(0.6931217908859253f, 0.6931217908859253f));
-  p = f32x2_fma(p, f, f32x2(0.9999992847442627f, 0.9999992847442627f));
+  uint64_t p = f32x2_fma(f, f32x2(0.009782912209630013f, 0.009782912209630013f), f32x2(0.055976882576942444f, 0.055976882576942444f));
+  p = f32x2_fma(p, f, f32x2(0.24020710587501526f, 0.24020710587501526f));
+  p = f32x2_fma(p, f, f32x2(0.6931136250495911f, 0.6931136250495911f));
+  p = f32x2_fma(p, f, f32x2(1.f, 1.f));
   const float2 y = f32x2_parts(p), n = f32x2_parts(t);
   return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
               for (int e = 0; e < 16; ++e) {
                 const uint64_t v = f32x2_fma(f32x2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), f32x2(args.scale_log2, args.scale_log2), f32x2(shift, shift));
                 float2 y;
-                if (e % kWidePoly == kWidePoly - 1) {  // what is masked gets 2^-126 here; a row with nothing else is looked after below
+                if (e % kWidePoly == kWidePoly - 1) {
                   y = exp2_poly(v);
                 } else {
                   y = f32x2_parts(v);
@@ -403,11 +404,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       const bool split = x->split != 0, whole = x->whole != 0, both = split && x->t1 > x->t0;
       const bool busy = G0 + (warp & 3) * 32 < x->rows, exists = G0 + row < x->rows;
       const int at = x->row0 + G0 + row, j = at / G;
-      // a row that sees nothing of this accumulator's positions (it sees the first so many of the request)
-      if (!exists || x->len - x->n + j + 1 <= x->t0 * kWideTile + (split ? w * kWideHalf : 0)) {
-        ref = -INFINITY;
-        sum = 0;
-      }
       if (count > 0) {
         wait_warp(&o_full[w], ph_o);
         ph_o ^= 1u;

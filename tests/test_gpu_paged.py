@@ -292,6 +292,24 @@ def test_attention_call_behind_call():
         assert_attention(out, p, hq, hkv)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("have,new", [(0, 2), (0, 64), (100, 150), (0, 300)])
+def test_later_tokens_have_no_weight_at_all(dtype, have, new):
+    """The greatest values that there are behind a row's own position leave its zeros as they are."""
+    hq, hkv, page = 8, 1, 64
+    q, k, v, table, total, cu = paged_problem(dtype, page, hq, hkv, [have], [new], seed=new)
+    half = have + new // 2
+    flat = torch.zeros(total[0], hkv, D, device="cuda", dtype=dtype)
+    flat[half:] = torch.finfo(dtype).max / 2
+    for c in range(ref.pages_of(total[0], page)):
+        m = min(page, total[0] - c * page)
+        v[table[0][c], :, :m] = flat[c * page:c * page + m].transpose(0, 1)
+    out = attend((q, k, v, table, total, cu), hq, hkv)
+    # Rows that see such values are not asked for more than their sign: before they are divided by the sum of the weights, outputs are sums of n
+    # weights of up to 2^8 times 2^127 in bf16, where fp32 ends at 2^128.
+    assert (out[:new // 2] == 0).all() and (out[new // 2:] > 0).all()
+
+
 def test_two_captured_graphs_share_a_workspace():
     """One of single tokens and one of chunks, replayed in turn with lengths that change between the replays."""
     hq, hkv = 8, 2
