@@ -315,10 +315,10 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
             v = make_float4(v.x + y.x * f, v.y + y.y * f, v.z + y.z * f, v.w + y.w * f);
           }
           if (whole) {
-            const float inv = l == 0 ? 0.f : 1 / l;  // a row that sees nothing
             const int j = row / G;
+            const float4 y = divided(v, l, all_see + j > 0);
             T* dst = static_cast<T*>(args.out) + (int64_t(first_row + j) * args.hq + int64_t(h) * G + (row - j * G)) * kAttnD + lane * 4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
           } else {
             if (lane == 0) *reinterpret_cast<float2*>(piece + 2 * row) = make_float2(m, l);
             *reinterpret_cast<float4*>(piece + 2 * kNarRows + row * kAttnD + lane * 4) = v;
@@ -342,10 +342,10 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
               const float* p = Piece<kNarRows>::slot(args, from + n, n == 0 ? 1 : 0);
               sum.add(__ldcg(reinterpret_cast<const float2*>(p + 2 * row)), __ldcg(reinterpret_cast<const float4*>(p + 2 * kNarRows + row * kAttnD + lane * 4)));
             }
-            const float inv = sum.l == 0 ? 0.f : 1 / sum.l;
             const int j = row / G;
+            const float4 y = divided(sum.o, sum.l, all_see + j > 0);
             T* dst = static_cast<T*>(args.out) + (int64_t(first_row + j) * args.hq + int64_t(h) * G + (row - j * G)) * kAttnD + lane * 4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(sum.o.x * inv, sum.o.y * inv), pack2<T>(sum.o.z * inv, sum.o.w * inv));
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
           }
         }
       }

@@ -216,14 +216,15 @@ __device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
   return x;
 }
+// NaN where one of them is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float m;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
   return m;
 }
 // 2^x for two values up to 127, without the special function unit: x = n + f with |f| <= 1/2, 2^f by the polynomial 1 + f q(f) of degree 4 whose
 // greatest relative error there is least (3.6e-6, found by Remez' exchange), n into the exponent.  From -127 down, -inf included, it is zero (the bits
-// of 1 less 127 in the exponent), between -127 and -126 what is below 2^-126; NaN gives what is not finite as a 16-bit weight.
+// of 1 less 127 in the exponent), between -127 and -126 what is below 2^-126; what NaN gives is no number to go by.
 __device__ __forceinline__ float2 exp2_poly(uint64_t x) {
   float2 v = f32x2_parts(x);
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.f));
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
             for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[e + 4], s[e + 8]);
 #pragma unroll
             for (int e = 12; e < kWideHalf; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], s[e], s[e + 1]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * args.scale_log2;
+            const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * args.scale_log2;
             if (__any_sync(0xffffffffu, top > ref + kWideSlack)) {
               const float now = fmaxf(ref, top);
               if (i > 0) {
@@ -394,7 +395,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
             tmem_st_wait();
             tc_fence_before_sync();
             const float2 a = f32x2_parts(f32x2_add(part[0], part[1]));
-            sum += a.x + a.y;
+            // A score of NaN or +inf (inf - inf) makes the row NaN.  The sum has to say so: exp2_poly does not.
+            sum = top < INFINITY ? sum + (a.x + a.y) : __int_as_float(0x7fffffff);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_ready[w][b]);
@@ -459,8 +461,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       }
       if ((!split || w == 0) && busy) {
         if (exists && !whole) *reinterpret_cast<float2*>(Piece<kWideRows>::slot(args, int(blockIdx.x), x->t0 > 0 ? 0 : 1) + 2 * (G0 + row)) = make_float2(ref, sum);
+        float none = 0;  // for a row without a weight
         if (whole) {
-          const float inv = sum == 0 ? 0.f : 1 / sum;  // a row that sees nothing
+          if (sum == 0) none = no_weight(x->len - x->n + j >= 0);
+          const float inv = sum == 0 ? 0.f : 1 / sum;
           f *= inv;
           g *= inv;
         }
@@ -468,12 +472,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         for (int c = 0; c < kAttnD; c += 32) {
           uint32_t o[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(none);
           if (count > 0) {
             tmem_ld_32cols(o_addr + uint32_t(c), o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = f != 0 && sum != 0 ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(f != 0 && sum != 0 ? __uint_as_float(o[e]) * f : none);
           }
           if (both) {
             uint32_t y[32];

@@ -266,6 +266,17 @@ __device__ __forceinline__ void zero_tail(const PagedArgs& a) {
       reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.hq * kAttnD)[v] = make_uint4(0, 0, 0, 0);
 }
 
+// What a row without a weight (a sum of zero) is: zero where it sees no position, 0 / 0 where it sees some and all their scores are -inf.
+__device__ __forceinline__ float no_weight(bool sees) { return sees ? __int_as_float(0x7fffffff) : 0.f; }
+__device__ __forceinline__ float4 divided(const float4& o, float l, bool sees) {
+  if (l == 0) {
+    const float x = no_weight(sees);
+    return make_float4(x, x, x, x);
+  }
+  const float inv = 1 / l;
+  return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
 // ---- the join ---------------------------------------------------------------------------------------------------------
 // Where an item starts in span c = blockIdx.x and goes on in the next, its pieces are weighted with 2^(maximum - greatest maximum) and added
 // in order.  Eight rows a CTA: a warp each, or, where there are many pieces, all warps for one row after the other.
@@ -302,10 +313,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     from = k <= spans ? a.starts[k] : Start{-1};
   }
   auto write = [&](const Joined& x, int row) {
-    const float inv = x.l == 0 ? 0.f : 1 / x.l;
     const int at = next.row0 + row, j = at / a.group;
+    const float4 y = divided(x.o, x.l, next.r.len - next.r.n + j >= 0);
     T* dst = static_cast<T*>(a.out) + (int64_t(next.r.row0 + j) * a.hq + int64_t(next.h) * a.group + (at - j * a.group)) * kAttnD + lane * 4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x.o.x * inv, x.o.y * inv), pack2<T>(x.o.z * inv, x.o.w * inv));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
   };
   auto gather = [&](int row, int first, int step) {
     Joined x;
