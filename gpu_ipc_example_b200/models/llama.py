@@ -307,6 +307,7 @@ class LlamaTP:
     @torch.no_grad()
     def probabilities(self, hidden: List[torch.Tensor], temperature: float = 1.0) -> torch.Tensor:
         """softmax(logits / temperature) over the whole vocabulary, [rows, vocab] in fp32, of hidden states of every local rank."""
+        self._check_temperature(temperature)
         logits = [x @ w.t() for x, w in zip(hidden, self.lm_head)]
         if self.nlocal < self.world:
             import torch.distributed as dist
@@ -316,21 +317,49 @@ class LlamaTP:
             logits = parts
         return torch.softmax(torch.cat(logits, -1).float() / temperature, -1)
 
+    def _check_verify(self, last, drafts, draft_probs, cache, accept, sample, temperature):
+        """What a speculative step refuses, before anything has changed."""
+        B, dev = cache.requests, cache.lens.device
+        if drafts.dim() != 2 or drafts.shape[0] != B or drafts.shape[1] > 1024:
+            raise ValueError(f"drafts must be [{B}, at most 1024], got {list(drafts.shape)}")
+        K = drafts.shape[1]
+        wanted = [("last", last, (B,), torch.int32 if last.dtype == torch.int32 else torch.int64), ("drafts", drafts, (B, K), torch.int64), ("accept", accept, (B, K), torch.float32),
+                  ("sample", sample, (B,), torch.float32)]
+        if draft_probs is not None:
+            wanted.append(("draft_probs", draft_probs, (B, K, self.cfg.vocab), torch.float32))
+            if draft_probs.dim() == 3 and draft_probs.stride(2) != 1:
+                raise ValueError("draft_probs must have contiguous words")
+        for name, t, shape, dtype in wanted:
+            if tuple(t.shape) != shape or t.dtype != dtype or t.device != dev:
+                raise ValueError(f"{name} must be {dtype} {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+        self._check_temperature(temperature)
+
+    @staticmethod
+    def _check_temperature(temperature):
+        if isinstance(temperature, (int, float)) and not temperature > 0:  # tensors are not looked at: that would wait for the GPU
+            raise ValueError(f"the temperature must be above 0, got {temperature} (greedy ids: next_ids)")
+
     @torch.no_grad()
     def verify(self, last: torch.Tensor, drafts: torch.Tensor, draft_probs: Optional[torch.Tensor], cache, accept: torch.Tensor, sample: torch.Tensor,
                temperature: float = 1.0):
         """A step of speculative decoding: `last` [requests] is every request's newest token (not in the cache yet), `drafts` [requests, K] what a
         draft model says comes next, with `draft_probs` [requests, K, vocab] (None: it is certain); accept [requests, K] and sample [requests] are
         uniform random numbers, the same on every rank.  Returns (tokens [requests, K + 1]: the accepted drafts and one more, then -1;
-        accepted [requests]).  The cache then holds `last` and the accepted drafts; the one more is the next `last`."""
+        accepted [requests]).  The cache then holds `last` and the accepted drafts; the one more is the next `last`.  A call that raises leaves
+        the cache's lengths and pages as they were."""
+        self._check_verify(last, drafts, draft_probs, cache, accept, sample, temperature)
         B, K = drafts.shape
         before = cache.lens.clone()
         batch = cache.extend(torch.full_like(before, K + 1), B * (K + 1), K + 1)
-        hidden = self.forward_paged(torch.cat([last[:, None], drafts], 1).view(-1), batch, cache)
-        probs = self.probabilities(hidden, temperature).view(B, K + 1, -1)
-        tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts, None, accept, sample)
-        # a step that found no room has added nothing
-        cache.trim(torch.minimum(cache.lens, before + accepted + 1))
+        try:
+            hidden = self.forward_paged(torch.cat([last[:, None], drafts], 1).view(-1), batch, cache)
+            probs = self.probabilities(hidden, temperature).view(B, K + 1, -1)
+            tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts.contiguous(), None, accept.contiguous(), sample.contiguous())
+            keep = torch.minimum(cache.lens, before + accepted + 1)  # a step that found no room has added nothing
+        except BaseException:
+            cache.trim(torch.minimum(cache.lens, before))
+            raise
+        cache.trim(keep)
         return tokens, accepted
 
     @torch.no_grad()
