@@ -345,8 +345,9 @@ class LlamaTP:
         """A step of speculative decoding: `last` [requests] is every request's newest token (not in the cache yet), `drafts` [requests, K] what a
         draft model says comes next, with `draft_probs` [requests, K, vocab] (None: it is certain); accept [requests, K] and sample [requests] are
         uniform random numbers, the same on every rank.  Returns (tokens [requests, K + 1]: the accepted drafts and one more, then -1;
-        accepted [requests]).  The cache then holds `last` and the accepted drafts; the one more is the next `last`.  A call that raises leaves
-        the cache's lengths and pages as they were."""
+        accepted [requests]).  The cache then holds `last` and the accepted drafts; the one more is the next `last`.  A step that found no room
+        (`cache.check()` says which) has changed nothing and answers nothing: all tokens and counts are -1.  A call that raises leaves the
+        cache's lengths and pages as they were."""
         self._check_verify(last, drafts, draft_probs, cache, accept, sample, temperature)
         B, K = drafts.shape
         before = cache.lens.clone()
@@ -355,7 +356,9 @@ class LlamaTP:
             hidden = self.forward_paged(torch.cat([last[:, None], drafts], 1).view(-1), batch, cache)
             probs = self.probabilities(hidden, temperature).view(B, K + 1, -1)
             tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts.contiguous(), None, accept.contiguous(), sample.contiguous())
-            keep = torch.minimum(cache.lens, before + accepted + 1)  # a step that found no room has added nothing
+            made = batch.cu_new[1:] > batch.cu_new[:-1]
+            tokens, accepted = tokens.masked_fill_(~made[:, None], -1), accepted.masked_fill_(~made, -1)
+            keep = torch.minimum(cache.lens, before + accepted + 1)
         except BaseException:
             cache.trim(torch.minimum(cache.lens, before))
             raise

@@ -5,11 +5,16 @@ import torch
 
 from gpu_ipc_example_b200 import Communicator
 from gpu_ipc_example_b200.models.llama import LlamaConfig, LlamaTP
-from gpu_ipc_example_b200.models.paged import PagedCache
+from gpu_ipc_example_b200.models.paged import PagedCache, PagedCacheError
 from test_gpu_paged_serving import ints, served
 
 pytestmark = pytest.mark.gpu
 K = 3
+
+
+def state(cache):
+    """Bits of all that a step changes; what stands behind a request's last token is of no account, but unchanged where nothing is written."""
+    return [c.clone() for c in (cache.k[0][0].view(torch.int16), cache.v[0][1].view(torch.int16), cache.block_table, cache.lens, cache.free_pages, cache.n_free)]
 
 
 def tables(cache):
@@ -31,6 +36,19 @@ def numbers(model, B, g):
     drafts = torch.multinomial(probs.view(B * K, -1), 1, generator=g).view(B, K)
     last = torch.randint(0, model.cfg.vocab, (B,), device="cuda", generator=g)
     return [last, drafts, probs, torch.rand(B, K, device="cuda", generator=g) * 0.5, torch.rand(B, device="cuda", generator=g)]
+
+
+def test_a_step_without_room_answers_nothing():
+    with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
+        model, cache, g = made(comm, [30, 10], pages=3)
+        keep = state(cache)
+        last, drafts, probs, accept, sample = numbers(model, 2, g)
+        for p in (probs, None):
+            tokens, accepted = model.verify(last, drafts, p, cache, torch.zeros_like(accept), sample)  # all drafts would be accepted
+            assert (tokens == -1).all() and (accepted == -1).all()
+            assert all(torch.equal(a, b) for a, b in zip(keep, state(cache)))
+        with pytest.raises(PagedCacheError, match="pages run out"):
+            cache.check()
 
 
 def test_refused_arguments_leave_the_cache_as_it_is():
