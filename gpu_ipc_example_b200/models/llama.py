@@ -317,7 +317,7 @@ class LlamaTP:
             logits = parts
         return torch.softmax(torch.cat(logits, -1).float() / temperature, -1)
 
-    def _check_verify(self, last, drafts, draft_probs, cache, accept, sample, temperature):
+    def _check_verify(self, last, drafts, draft_probs, cache, accept, sample, temperature, draft_lens):
         """What a speculative step refuses, before anything has changed."""
         B, dev = cache.requests, cache.lens.device
         if drafts.dim() != 2 or drafts.shape[0] != B or drafts.shape[1] > 1024:
@@ -325,6 +325,8 @@ class LlamaTP:
         K = drafts.shape[1]
         wanted = [("last", last, (B,), torch.int32 if last.dtype == torch.int32 else torch.int64), ("drafts", drafts, (B, K), torch.int64), ("accept", accept, (B, K), torch.float32),
                   ("sample", sample, (B,), torch.float32)]
+        if draft_lens is not None:
+            wanted.append(("draft_lens", draft_lens, (B,), torch.int32))
         if draft_probs is not None:
             wanted.append(("draft_probs", draft_probs, (B, K, self.cfg.vocab), torch.float32))
             if draft_probs.dim() == 3 and draft_probs.stride(2) != 1:
@@ -341,21 +343,33 @@ class LlamaTP:
 
     @torch.no_grad()
     def verify(self, last: torch.Tensor, drafts: torch.Tensor, draft_probs: Optional[torch.Tensor], cache, accept: torch.Tensor, sample: torch.Tensor,
-               temperature: float = 1.0):
+               temperature: float = 1.0, draft_lens: Optional[torch.Tensor] = None):
         """A step of speculative decoding: `last` [requests] is every request's newest token (not in the cache yet), `drafts` [requests, K] what a
         draft model says comes next, with `draft_probs` [requests, K, vocab] (None: it is certain); accept [requests, K] and sample [requests] are
-        uniform random numbers, the same on every rank.  Returns (tokens [requests, K + 1]: the accepted drafts and one more, then -1;
-        accepted [requests]).  The cache then holds `last` and the accepted drafts; the one more is the next `last`.  A step that found no room
-        (`cache.check()` says which) has changed nothing and answers nothing: all tokens and counts are -1.  A call that raises leaves the
+        uniform random numbers, the same on every rank.  draft_lens [requests] int32: request i has the first draft_lens[i] drafts (those behind are
+        not looked at), and with -1 no part in the step, as a slot of the cache without a request has to have; None: all have K.
+
+        Returns (tokens [requests, K + 1]: the accepted drafts and one more, then -1; accepted [requests], -1 for requests without a part).  The
+        cache then holds `last` and the accepted drafts; the one more is the next `last`.  A step that found no room for all its tokens
+        (`cache.check()` says which kind) has changed nothing and answers nothing: all tokens and counts are -1.  A call that raises leaves the
         cache's lengths and pages as they were."""
-        self._check_verify(last, drafts, draft_probs, cache, accept, sample, temperature)
+        self._check_verify(last, drafts, draft_probs, cache, accept, sample, temperature, draft_lens)
         B, K = drafts.shape
+        rows = B * (K + 1)
         before = cache.lens.clone()
-        batch = cache.extend(torch.full_like(before, K + 1), B * (K + 1), K + 1)
+        new = torch.full_like(before, K + 1) if draft_lens is None else draft_lens.clamp(-1, K) + 1
+        batch = cache.extend(new, rows, K + 1)
         try:
-            hidden = self.forward_paged(torch.cat([last[:, None], drafts], 1).view(-1), batch, cache)
+            ids = torch.cat([last[:, None], drafts], 1).view(-1)
+            if draft_lens is not None:  # request behind request, and back
+                at = batch.cu_new[:-1, None] + torch.arange(K + 1, device=self.dev)
+                at = torch.where(at < batch.cu_new[1:, None], at, rows).view(-1).long()  # one place more takes what is no token
+                ids = ids.new_zeros(rows + 1).scatter_(0, at, ids)[:rows]
+            hidden = self.forward_paged(ids, batch, cache)
+            if draft_lens is not None:
+                hidden = [x[at.clamp(max=rows - 1)] for x in hidden]
             probs = self.probabilities(hidden, temperature).view(B, K + 1, -1)
-            tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts.contiguous(), None, accept.contiguous(), sample.contiguous())
+            tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts.contiguous(), draft_lens, accept.contiguous(), sample.contiguous())
             made = batch.cu_new[1:] > batch.cu_new[:-1]
             tokens, accepted = tokens.masked_fill_(~made[:, None], -1), accepted.masked_fill_(~made, -1)
             keep = torch.minimum(cache.lens, before + accepted + 1)

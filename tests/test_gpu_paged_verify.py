@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import paged_reference as ref
 from gpu_ipc_example_b200 import Communicator
 from gpu_ipc_example_b200.models.llama import LlamaConfig, LlamaTP
 from gpu_ipc_example_b200.models.paged import PagedCache, PagedCacheError
@@ -60,7 +61,7 @@ def test_refused_arguments_leave_the_cache_as_it_is():
         for change in (dict(draft_probs=probs.half()), dict(draft_probs=probs[:, :2]), dict(draft_probs=probs[..., :100]), dict(draft_probs=probs.transpose(1, 2)),
                        dict(accept=accept.double()), dict(accept=accept[:, :2]), dict(sample=sample[:1]), dict(sample=sample.cpu()), dict(last=last[:1]),
                        dict(last=last.float()), dict(drafts=drafts.int()), dict(drafts=drafts[0]), dict(drafts=drafts[:1], draft_probs=None, accept=accept[:1]),
-                       dict(temperature=0.0), dict(temperature=float("nan"))):
+                       dict(temperature=0.0), dict(temperature=float("nan")), dict(draft_lens=ints([1, 1, 1])), dict(draft_lens=ints([1, 1], torch.int64))):
             with pytest.raises((ValueError, RuntimeError)):
                 model.verify(**{**good, **change})
             assert all(torch.equal(a, b) for a, b in zip(keep, tables(cache))), change.keys()
@@ -83,3 +84,72 @@ def test_a_step_that_fails_midway_leaves_no_tokens(monkeypatch):
             model.verify(*args[:3], cache, *args[3:])
         assert all(torch.equal(a, b) for a, b in zip(keep, tables(cache)))
         cache.check()
+
+
+@pytest.mark.parametrize("certain", [False, True])
+def test_requests_with_fewer_drafts_and_without_any_part(certain):
+    """Slot 1 has no request, slot 2 has room for two tokens and one draft, slot 4 none at all, slot 5 sits the step out."""
+    lens, count = [17, 0, 62, 9, 16, 33], [K, -1, 1, 2, 0, -1]
+    with Communicator.virtual(2, 0, staging_bytes=64 << 20) as comm:
+        prompts = [n if n else 1 for n in lens]
+        (model, cache, g), (_, other, _) = made(comm, prompts), made(comm, prompts)
+        for c in (cache, other):
+            c.trim(ints(lens))  # slot 1: a request that is done
+        last, drafts, probs, accept, sample = numbers(model, 6, g)
+        padded, told = drafts.clone(), last.clone()
+        for i, n in enumerate(count):
+            padded[i, max(n, 0):] = -1  # whatever stands there
+            if n < 0:
+                told[i] = -1
+        p = None if certain else probs
+        tokens, accepted = model.verify(told, padded, p, cache, accept, sample, draft_lens=ints(count))
+        cache.check()
+        comm.check()
+        # the same by hand: the tokens of the requests that take part, one request after the other
+        ids = [torch.cat([last[i:i + 1], drafts[i, :n]]) if n >= 0 else last[:0] for i, n in enumerate(count)]
+        batch = other.extend(ints([len(x) for x in ids]), 6 * (K + 1), K + 1)
+        hidden = model.forward_paged(torch.cat(ids + [last.new_zeros(6 * (K + 1) - sum(map(len, ids)))]), batch, other)
+        flat = model.probabilities(hidden).cpu()
+        at, target = 0, torch.zeros(6, K + 1, model.cfg.vocab)
+        for i, x in enumerate(ids):
+            target[i, :len(x)] = flat[at:at + len(x)]
+            at += len(x)
+        want, n_want = ref.verify(target, None if certain else probs.cpu(), drafts.cpu(), ints(count).cpu(), accept.cpu(), sample.cpu())
+        for i, n in enumerate(count):
+            if n < 0:
+                want[i], n_want[i] = -1, -1
+        assert torch.equal(tokens.cpu(), want) and torch.equal(accepted.cpu(), n_want)
+        assert cache.lens.tolist() == [n + a + 1 for n, a in zip(lens, n_want.tolist())]
+        assert int(cache.n_free) == 20 - sum(ref.pages_of(n, 16) for n in cache.lens.tolist())
+
+
+def test_a_captured_speculative_step():
+    """Draft lengths change between the replays, and the pages run out in the end."""
+    with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
+        (model, cache, g), (_, other, _) = made(comm, [5, 30, 12], pages=7), made(comm, [5, 30, 12], pages=7)
+        args, count = numbers(model, 3, g), ints([K, 0, -1])
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        refused = 0
+        with torch.cuda.stream(stream):
+            before = cache.lens.clone()
+            model.verify(*args[:3], cache, *args[3:], draft_lens=count)
+            cache.trim(before)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                got = model.verify(*args[:3], cache, *args[3:], draft_lens=count)
+            for step in range(40):
+                for a, b in zip(args, numbers(model, 3, g)):
+                    a.copy_(b)
+                count.copy_(ints([step % (K + 2) - 1, K, (step + 2) % (K + 2) - 1]))
+                graph.replay()
+                want = model.verify(*args[:3], other, *args[3:], draft_lens=count)
+                stream.synchronize()
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+                assert torch.equal(cache.lens, other.lens)
+                refused += bool((want[1] == -1).all())
+        assert refused
+        with pytest.raises(PagedCacheError, match="pages run out"):
+            cache.check()
+        del graph
