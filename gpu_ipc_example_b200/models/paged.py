@@ -8,7 +8,7 @@
 
 Lengths, the block table and the list of free pages are on the GPU and no call here reads them back, so steps of one number of rows can be
 captured in a CUDA graph; all calls on one cache follow one another, on a stream or by events.  What a call cannot do (no pages left, a
-request beyond `max_len`, more tokens than rows) it leaves undone and says so in a word of its own; `check()`, which waits for the GPU, raises it.
+request beyond its row of the table, more tokens than rows) it leaves undone and says so in a word of its own; `check()`, which waits for the GPU, raises it.
 
 The reference has no model code and no cache.
 """
@@ -41,8 +41,8 @@ class PagedBatch:
 
 class PagedCache:
     def __init__(self, model, requests: int, max_len: int, pages: int, page: int = 64):
-        """Room for `requests` requests of up to `max_len` tokens, in `pages` pages of `page` (16, 32, 64 or 128) positions that they
-        share: `pages` bounds what all of them hold together."""
+        """Room for `requests` requests of up to `max_len` tokens (rounded up to whole pages), in `pages` pages of `page` (16, 32, 64 or 128)
+        positions that they share: `pages` bounds what all of them hold together."""
         if not model.kernels:
             raise ValueError("a paged cache is for the decode kernels: head_dim 128 and 1, 2, 4 or 8 query heads per KV head")
         if page not in (16, 32, 64, 128):
@@ -60,15 +60,17 @@ class PagedCache:
         self._said = torch.zeros(1, dtype=torch.int32, device=dev)  # all that extend and trim could not do
         # Scratch of the attention for steps of any size: a captured step goes on using it, so it never makes room for a larger one.
         device = dev.index if dev.index is not None else torch.cuda.current_device()
-        need = load().paged_attention_workspace_bytes(model.hq // model.hkv, max(1, min(requests * max_len, 1 << 20)), device)
+        self.max_len = self.block_table.shape[1] * page
+        need = load().paged_attention_workspace_bytes(model.hq // model.hkv, max(1, min(self.max_len, 1 << 20)), device)
         self.workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
 
     def extend(self, new_lens: torch.Tensor, rows: int, max_new: Optional[int] = None) -> PagedBatch:
         """Room for new_lens[i] more tokens of request i ([requests] int32 on the GPU); `rows` is the size of the batch that they are the first
-        rows of, `max_new` what no new_lens is above (the number of rows, if it is not known)."""
+        rows of, `max_new` what no new_lens is above (as many as there are rows, if it is not known: a step of single tokens should say 1, as
+        the attention has a faster kernel for requests of up to 16 (new token, query head) pairs a KV head)."""
         cu, slots, positions, status = torch.ops.b200ipc.paged_extend(self.block_table, self.lens, new_lens, self.free_pages, self.n_free, self.page, rows)
         self._said.bitwise_or_(status)
-        return PagedBatch(cu, slots, positions, max(1, rows if max_new is None else min(max_new, rows)))
+        return PagedBatch(cu, slots, positions, max(1, min(rows if max_new is None else max_new, rows, self.max_len)))
 
     def trim(self, keep_lens: torch.Tensor) -> None:
         """Request i keeps its first keep_lens[i] tokens; pages that are not needed for them are free again."""

@@ -153,3 +153,16 @@ def test_a_captured_speculative_step():
         with pytest.raises(PagedCacheError, match="pages run out"):
             cache.check()
         del graph
+
+
+def test_a_small_cache_takes_padded_batches():
+    """Fewer tokens fit the cache than the batch has rows: the rows say nothing of how long a request is."""
+    with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
+        model = LlamaTP(LlamaConfig.tiny128(), comm, batch=1, max_ctx=8, fusion="allreduce", seed=3)
+        tokens = torch.arange(40, device="cuda")
+        hidden = []
+        for max_len in (8, 4000):
+            cache = PagedCache(model, requests=1, max_len=max_len, pages=4, page=16)
+            hidden.append(model.forward_paged(tokens, cache.extend(ints([8]), 40), cache)[0][:8].clone())
+            cache.check()
+        torch.testing.assert_close(hidden[0].float(), hidden[1].float(), atol=6e-2, rtol=5e-2)  # another kernel, perhaps
