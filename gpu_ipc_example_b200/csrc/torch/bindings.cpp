@@ -695,13 +695,6 @@ void check_ints(const at::Tensor& t, at::ScalarType type, at::IntArrayRef sizes,
 }
 // Past the dispatcher: an output costs a third of a microsecond.
 at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt); }
-// A tensor of `whole`'s memory, `offset` elements of its own type from the start on.
-at::Tensor part_of(const at::Tensor& whole, int64_t offset, int64_t n, at::ScalarType type) {
-  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
-  t.unsafeGetTensorImpl()->set_storage_offset(offset);
-  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-  return t;
-}
 void check_one_device(std::initializer_list<const at::Tensor*> ts, const char* op) {
   const at::Device d = (*ts.begin())->device();
   for (const at::Tensor* t : ts)
@@ -737,10 +730,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_extend_op(at::T
       if (t != w) check_apart(*w, *t, op);
   }
   c10::cuda::CUDAGuard guard(table.device());
-  // the four outputs are one allocation: three more would be a sixth of the call's host time
-  const at::Tensor whole = empty_on(table, {rows + (rows + B + 3) / 2}, at::kLong);
-  at::Tensor slots = part_of(whole, 0, rows, at::kLong), positions = part_of(whole, 2 * rows, rows, at::kInt), cu = part_of(whole, 3 * rows, B + 1, at::kInt),
-             status = part_of(whole, 3 * rows + B + 1, 1, at::kInt);
+  at::Tensor cu = empty_on(table, {B + 1}, at::kInt), slots = empty_on(table, {rows}, at::kLong), positions = empty_on(table, {rows}, at::kInt),
+             status = empty_on(table, {1}, at::kInt);
   paged_extend(table.data_ptr<int>(), lens.data_ptr<int>(), new_lens.data_ptr<int>(), free_pages.data_ptr<int>(), n_free.data_ptr<int>(),
                cu.data_ptr<int>(), slots.data_ptr<int64_t>(), positions.data_ptr<int>(), status.data_ptr<int>(), int(B), int(table.size(1)),
                int(free_pages.numel()), int(page), int(rows), at::cuda::getCurrentCUDAStream(table.get_device()));

@@ -1,4 +1,5 @@
 """Speculative steps of the decoder where not every request takes part, has all drafts or finds room, and where the call is refused."""
+import io
 
 import pytest
 import torch
@@ -166,3 +167,19 @@ def test_a_small_cache_takes_padded_batches():
             hidden.append(model.forward_paged(tokens, cache.extend(ints([8]), 40), cache)[0][:8].clone())
             cache.check()
         torch.testing.assert_close(hidden[0].float(), hidden[1].float(), atol=6e-2, rtol=5e-2)  # another kernel, perhaps
+
+
+def test_what_extend_returns_has_memory_of_its_own():
+    with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
+        model, cache, _ = made(comm, [7, 20])
+        batch = cache.extend(ints([3, 1]), 6, 3)
+        out = (batch.cu_new, batch.slots, batch.positions)
+        want = [t.tolist() for t in out]
+        assert len({t.untyped_storage().data_ptr() for t in out}) == 3
+        file = io.BytesIO()
+        torch.save(out, file)
+        file.seek(0)
+        assert [t.tolist() for t in torch.load(file)] == want
+        status = torch.ops.b200ipc.paged_extend(cache.block_table, cache.lens, ints([0, 0]), cache.free_pages, cache.n_free, 16, 1)[3]
+        status.resize_(64).fill_(-5)
+        assert [t.tolist() for t in out] == want
