@@ -187,9 +187,13 @@ __global__ void __launch_bounds__(kTabThreads) paged_trim_kernel(int* table, int
   }
 }
 
+constexpr size_t extend_smem(int requests) { return size_t(3 * requests + 2) * sizeof(int); }
+constexpr size_t trim_smem(int requests) { return size_t(2 * requests + 1) * sizeof(int); }
+
+// `most`: of a call with as many requests as there can be.  The limit is always set to that, as another thread may be about to launch.
 template <typename... Params, typename... Args>
-void launch_one_cluster(void (*kernel)(Params...), int ctas, size_t smem, cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024) B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+void launch_one_cluster(void (*kernel)(Params...), int ctas, size_t smem, size_t most, cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024) B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(ctas));
   cfg.blockDim = dim3(kTabThreads);
@@ -218,18 +222,16 @@ void launch_one_cluster(void (*kernel)(Params...), int ctas, size_t smem, cudaSt
 void paged_extend(int* table, int* lens, const int* new_lens, const int* free_pages, int* n_free, int* cu_new, int64_t* slots, int* positions,
                   int* status, int requests, int width, int capacity, int page, int rows, cudaStream_t stream) {
   B200_REQUIRE(requests >= 1 && requests <= kPagedMaxRequests && width >= 1 && page >= 1 && rows >= 0 && capacity >= 0, "paged_extend: bad sizes");
-  const size_t smem = size_t(3 * requests + 2) * sizeof(int);
-  launch_one_cluster(paged_extend_kernel, rows >= kTabWide ? 8 : 1, smem, stream, table, lens, new_lens, free_pages, n_free, cu_new, slots, positions,
-                     status, requests, width, capacity, page, rows);
+  launch_one_cluster(paged_extend_kernel, rows >= kTabWide ? 8 : 1, extend_smem(requests), extend_smem(kPagedMaxRequests), stream, table, lens, new_lens,
+                     free_pages, n_free, cu_new, slots, positions, status, requests, width, capacity, page, rows);
 }
 
 void paged_trim(int* table, int* lens, const int* keep_lens, int* free_pages, int* n_free, int* status, int requests, int width, int capacity,
                 int page, cudaStream_t stream) {
   B200_REQUIRE(requests >= 1 && requests <= kPagedMaxRequests && width >= 1 && page >= 1 && capacity >= 0, "paged_trim: bad sizes");
-  const size_t smem = size_t(2 * requests + 1) * sizeof(int);
   // at most every page of the table comes back
-  launch_one_cluster(paged_trim_kernel, int64_t(requests) * width >= 8 * kTabWide ? 8 : 1, smem, stream, table, lens, keep_lens, free_pages, n_free,
-                     status, requests, width, capacity, page);
+  launch_one_cluster(paged_trim_kernel, int64_t(requests) * width >= 8 * kTabWide ? 8 : 1, trim_smem(requests), trim_smem(kPagedMaxRequests), stream, table,
+                     lens, keep_lens, free_pages, n_free, status, requests, width, capacity, page);
 }
 
 }  // namespace b200ipc

@@ -1,11 +1,13 @@
 """Speculative steps of the decoder where not every request takes part, has all drafts or finds room, and where the call is refused."""
 import io
+import threading
 
 import pytest
 import torch
 
 import paged_reference as ref
 from gpu_ipc_example_b200 import Communicator
+from gpu_ipc_example_b200._ext import load
 from gpu_ipc_example_b200.models.llama import LlamaConfig, LlamaTP
 from gpu_ipc_example_b200.models.paged import PagedCache, PagedCacheError
 from test_gpu_paged_serving import ints, served
@@ -183,3 +185,32 @@ def test_what_extend_returns_has_memory_of_its_own():
         status = torch.ops.b200ipc.paged_extend(cache.block_table, cache.lens, ints([0, 0]), cache.free_pages, cache.n_free, 16, 1)[3]
         status.resize_(64).fill_(-5)
         assert [t.tolist() for t in out] == want
+
+
+@pytest.mark.parametrize("few,many", [(4200, 8192), (6500, 8192)])  # above 48 KB of shared memory for extend alone, and for trim as well
+def test_threads_with_different_numbers_of_requests(few, many):
+    """Launches of both sizes from two host threads: what one of them asks of the kernel does not take from the other."""
+    failed = []
+
+    def steps(requests):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                table, lens, none = torch.full((requests, 1), -1, dtype=torch.int32, device="cuda"), ints([0] * requests), ints([0] * requests)
+                free, n_free = torch.arange(requests, dtype=torch.int32, device="cuda"), ints([requests])
+                for i in range(20000):
+                    if i % 2:
+                        torch.ops.b200ipc.paged_trim(table, lens, none, free, n_free, 16)
+                    else:
+                        torch.ops.b200ipc.paged_extend(table, lens, none, free, n_free, 16, 1)
+                    if i % 500 == 0:
+                        torch.cuda.current_stream().synchronize()
+        except Exception as e:  # of a thread
+            failed.append(e)
+
+    load()
+    threads = [threading.Thread(target=steps, args=(n,)) for n in (few, many)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed[0]
