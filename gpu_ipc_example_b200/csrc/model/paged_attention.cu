@@ -90,7 +90,8 @@ size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count) {
 }
 
 void paged_attention(DType t, const void* q, int64_t row_stride, const void* kcache, const void* vcache, const int* table, const int* lens,
-                     const int* cu_new, void* out, void* workspace, const PagedAttentionShape& s, int sm_count, cudaStream_t stream) {
+                     const int* cu_new, void* out, void* workspace, const PagedAttentionShape& s, int sm_count, uint64_t timeout_ns, uint32_t flags,
+                     cudaStream_t stream) {
   PagedArgs a{};
   a.tma_k = cache_map(t, kcache, s);
   a.tma_v = cache_map(t, vcache, s);
@@ -111,6 +112,8 @@ void paged_attention(DType t, const void* q, int64_t row_stride, const void* kca
   a.width = s.width;
   a.pages = s.pages;
   a.scale_log2 = 1.4426950408889634f / sqrtf(float(kAttnD));
+  a.timeout_ns = timeout_ns;
+  a.mute = (flags & kMuteSends) != 0;
   (t == DType::F16 ? run<__half> : run<__nv_bfloat16>)(a, s, static_cast<char*>(workspace) + kHead, sm_count, stream);
 }
 

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
   find_span<kNarThreads>(
       args, [&](const Request& r) { return cut.length(r); }, [&](const Request& r, int i, uint64_t o) { return cut.place(r, i, o); }, kNarLeast, s_sum, s_span, &s_axis);
   __syncthreads();
-  QueueEnd<Items, NarrowItem> items{s_queue, abort_flag};
+  QueueEnd<Items, NarrowItem> items{s_queue, abort_flag, args.timeout_ns};
 
   if (warp == kNarWarps + 1) {
     // ---- the walk ------------------------------------------------------------------------------------------------------------
@@ -133,10 +133,11 @@ __global__ void __launch_bounds__(kNarThreads, 1) paged_narrow_kernel(const __gr
         const int n = min(boxes, (len - t * kNarTile + box - 1) >> box_log);  // boxes that hold positions of the request
         items.wait_warp(&empty[st], ph ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) break;
-        if (lane == 0) mbar_expect_tx(&full[st], uint32_t(n << box_log) * kAttnD * 4u);
+        const int sent = args.mute && blockIdx.x == 0 && issued == 0 ? 0 : n;
+        if (lane == 0 && sent > 0) mbar_expect_tx(&full[st], uint32_t(n << box_log) * kAttnD * 4u);
         __syncwarp();
         unsigned char* dst = ring + st * 2 * kNarTileBytes;
-        for (int k = 0; k < n; ++k, dst += box * 128) {
+        for (int k = 0; k < sent; ++k, dst += box * 128) {
           const int row = __shfl_sync(0xffffffffu, at, k);
           if (elect_one()) {
             tma_load_2d(dst, &args.tma_k, &full[st], 0, row);

@@ -51,10 +51,11 @@ constexpr int kPagedMoreNew = 2;  // a request had more new tokens than max_new:
 // an infinity or NaN among the values of a token may reach all rows of its request (0 x inf), as in any masked product.  Outputs are fp32
 // sums of weights of up to 2^8 times values before they are divided: values of bf16 of 2^120 / positions and more may overflow there.
 // The workspace is zero before the first call and kept between calls, which follow one another; it serves calls of every shape that it is
-// large enough for.
+// large enough for.  `timeout_ns` bounds every wait inside the kernels.  Of the flags kMuteSends is known: one CTA leaves out its first copies, so the
+// waits for these run out.
 size_t paged_attention_workspace_bytes(int group, int max_new, int sm_count);
 void paged_attention(DType t, const void* q, int64_t row_stride, const void* kcache, const void* vcache, const int* table, const int* lens,
-                     const int* cu_new, void* out, void* workspace, const PagedAttentionShape& s, int sm_count, cudaStream_t stream);
+                     const int* cu_new, void* out, void* workspace, const PagedAttentionShape& s, int sm_count, uint64_t timeout_ns, uint32_t flags, cudaStream_t stream);
 
 struct VerifyShape {
   int requests, drafts;

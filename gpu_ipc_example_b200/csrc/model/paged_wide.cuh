@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
-  QueueEnd<Items, WideItem> items{s_queue, abort_flag};
+  QueueEnd<Items, WideItem> items{s_queue, abort_flag, args.timeout_ns};
   auto wait = [&](uint64_t* bar, uint32_t parity) { items.wait(bar, parity); };
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { items.wait_warp(bar, parity); };
 
@@ -505,10 +505,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
       auto load = [&](const CUtensorMap* map, int at, int n) {
         wait_warp(&kv_empty[st], ph ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) return;
-        if (lane == 0) mbar_expect_tx(&kv_full[st], uint32_t(n << box_log) * kAttnD * 2u);
+        const int sent = args.mute && blockIdx.x == 0 && issued == 0 ? 0 : n;
+        if (lane == 0 && sent > 0) mbar_expect_tx(&kv_full[st], uint32_t(n << box_log) * kAttnD * 2u);
         __syncwarp();
         unsigned char* dst = ring + st * kWideTileBytes;
-        for (int k = 0; k < n; ++k, dst += box * 128) {
+        for (int k = 0; k < sent; ++k, dst += box * 128) {
           const int row = __shfl_sync(0xffffffffu, at, k);
           if (elect_one()) {
             tma_load_2d(dst, map, &kv_full[st], 0, row);
@@ -616,7 +617,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
             if ((idle & 1023u) == 1023u) {  // nothing for a while
               const uint64_t now = globaltimer_ns();
               if (idle == 1023u) since = now;
-              if (*abort_flag || now - since > kPagedTimeoutNs) {
+              if (*abort_flag || now - since > args.timeout_ns) {
                 *abort_flag = 1;
                 break;
               }

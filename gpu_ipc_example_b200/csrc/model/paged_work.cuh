@@ -19,7 +19,6 @@
 
 namespace b200ipc {
 
-constexpr uint64_t kPagedTimeoutNs = 2000000000;  // a wait inside a CTA takes microseconds
 constexpr int kPagedQueue = 4;                    // items handed out ahead
 
 struct Request {
@@ -54,6 +53,8 @@ struct PagedArgs {
   int page_log, width;  // positions of a page: a power of two
   int64_t pages;
   int q_boxes;      // whether tma_q is there: 128 is a multiple of the group
+  uint64_t timeout_ns;  // of one wait inside a CTA, which takes microseconds
+  int mute;         // CTA 0's first copies into its ring are left out (failure injection)
   float scale_log2;
 };
 
@@ -189,9 +190,10 @@ template <typename Q, typename Item>
 struct QueueEnd {
   Q& q;
   volatile int* abort_flag;
+  uint64_t timeout_ns;
   uint32_t at = 0, ph = 0;
   __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
-    if (!mbar_try_wait(bar, parity) && !*abort_flag) mbar_wait(bar, parity, abort_flag, kPagedTimeoutNs);
+    if (!mbar_try_wait(bar, parity) && !*abort_flag) mbar_wait(bar, parity, abort_flag, timeout_ns);
   }
   // The same by all lanes of a warp, which leave it together: what follows may be instructions of the whole warp.
   __device__ __forceinline__ void wait_warp(uint64_t* bar, uint32_t parity) {
@@ -225,16 +227,18 @@ struct QueueEnd {
     mbar_arrive(&q.empty[at]);
     step();
   }
-  // false when nothing more is wanted
+  // false when nothing more is wanted.  Behind a wait that ran out the place may still be read, so it stays as it is: half of one item and half of
+  // another would be rows that are not there.
   __device__ __forceinline__ bool put(const Item& x) {
     wait_warp(&q.empty[at], ph ^ 1u);
+    if (__any_sync(0xffffffffu, *abort_flag)) return false;
     if ((threadIdx.x & 31) == 0) {
       q.items[at] = x;
       mbar_arrive(&q.full[at]);
     }
     __syncwarp();
     step();
-    return x.valid && !__any_sync(0xffffffffu, *abort_flag);
+    return x.valid != 0;
   }
 };
 

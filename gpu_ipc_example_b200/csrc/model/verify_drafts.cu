@@ -6,8 +6,8 @@
 //   zero), p_n where there is no draft n; it is the first word whose running sum is above sample * (sum of the weights).
 //
 // Products, differences and sums are taken in 64 bits: a product of two fp32 numbers is exact there, and a running sum over a vocabulary
-// is good to 1e-13, so that the words do not depend on the order of the additions (in 32 bits one draw in a hundred would).  NaN counts
-// as a probability of zero: every comparison with it fails.
+// is good to 1e-13, so that the words do not depend on the order of the additions (in 32 bits one draw in a hundred would).  With NaN every
+// comparison fails: a word of NaN has no weight in p, nor in max(p - q, 0) where either is NaN, and a draft whose p or q is NaN is turned down.
 //
 // Bound by memory: of all the rows one of p and one of q is read, 8 bytes a word.  A request is a cluster of CTAs, each with a piece of
 // the vocabulary, each of its warps with a run of it; the sums of all warps are exchanged through distributed shared memory, every CTA

@@ -796,7 +796,7 @@ int64_t paged_workspace_bytes(int64_t group, int64_t max_new, int64_t device) {
 }
 
 at::Tensor paged_attention_op(at::Tensor q, at::Tensor kcache, at::Tensor vcache, at::Tensor table, at::Tensor lens, at::Tensor cu_new, at::Tensor workspace,
-                              int64_t hq, int64_t hkv, int64_t max_new) {
+                              int64_t hq, int64_t hkv, int64_t max_new, int64_t timeout_ms, int64_t flags) {
   constexpr const char* op = "paged_attention";
   check_paged_cache(q, hq * 128, kcache, vcache, hq, hkv, op);
   const int64_t page = kcache.size(2);
@@ -808,6 +808,7 @@ at::Tensor paged_attention_op(at::Tensor q, at::Tensor kcache, at::Tensor vcache
   TORCH_CHECK(max_new >= 1 && max_new < (int64_t(1) << 30), "b200ipc: paged_attention: max_new must be at least 1, got ", max_new);
   TORCH_CHECK(hq / hkv <= 64, "b200ipc: paged_attention: at most 64 query heads per KV head, got ", hq / hkv);
   TORCH_CHECK(q.size(0) * (hq / hkv) < (int64_t(1) << 30), "b200ipc: paged_attention: too many rows");
+  TORCH_CHECK(timeout_ms >= 1 && timeout_ms <= 60000, "b200ipc: paged_attention: timeout_ms must be 1 to 60000, got ", timeout_ms);
   check_one_device({&q, &kcache, &vcache, &table, &lens, &cu_new, &workspace}, op);
   TORCH_CHECK(workspace.is_contiguous() && int64_t(workspace.nbytes()) >= paged_workspace_bytes(hq / hkv, max_new, q.get_device()) &&
                   (reinterpret_cast<uintptr_t>(workspace.data_ptr()) & 255) == 0,
@@ -818,7 +819,8 @@ at::Tensor paged_attention_op(at::Tensor q, at::Tensor kcache, at::Tensor vcache
   if (q.size(0) == 0) return out;
   const PagedAttentionShape s{int(q.size(0)), int(table.size(0)), int(hq), int(hkv), int(page), int(table.size(1)), kcache.size(0), int(std::min(max_new, q.size(0)))};
   paged_attention(dtype_of(q), q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), table.data_ptr<int>(), lens.data_ptr<int>(),
-                  cu_new.data_ptr<int>(), out.data_ptr(), workspace.data_ptr(), s, sm_count_of(q.get_device()), at::cuda::getCurrentCUDAStream(q.get_device()));
+                  cu_new.data_ptr<int>(), out.data_ptr(), workspace.data_ptr(), s, sm_count_of(q.get_device()), uint64_t(timeout_ms) * 1000000u, uint32_t(flags),
+                  at::cuda::getCurrentCUDAStream(q.get_device()));
   return out;
 }
 
@@ -1116,7 +1118,7 @@ TORCH_LIBRARY(b200ipc, m) {
   m.def("rope_paged_append(Tensor qkv, Tensor(a!) kcache, Tensor(b!) vcache, Tensor slots, Tensor positions, int hq, int hkv, float theta) -> Tensor",
         &rope_paged_append_op);
   m.def("paged_attention(Tensor q, Tensor kcache, Tensor vcache, Tensor block_table, Tensor lens, Tensor cu_new, Tensor(a!) workspace, int hq, "
-        "int hkv, int max_new) -> Tensor", &paged_attention_op);
+        "int hkv, int max_new, int timeout_ms=2000, int flags=0) -> Tensor", &paged_attention_op);
   m.def("verify_drafts(Tensor target_probs, Tensor? draft_probs, Tensor draft_tokens, Tensor? draft_lens, Tensor accept, Tensor sample) -> "
         "(Tensor, Tensor)", &verify_drafts_op);
   m.def("rmsnorm(Tensor x, Tensor gamma, float eps) -> Tensor", &rmsnorm_op);

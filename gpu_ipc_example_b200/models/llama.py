@@ -297,7 +297,8 @@ class LlamaTP:
             for i, qkv in enumerate(self._linear(normed, [w[l] for w in self.wqkv])):
                 k, v = cache.k[i][l], cache.v[i][l]
                 q = ops.rope_paged_append(qkv, k, v, batch.slots, batch.positions, self.hq, self.hkv, cfg.rope_theta)
-                attn_out.append(ops.paged_attention(q, k, v, cache.block_table, cache.lens, batch.cu_new, ws, self.hq, self.hkv, batch.max_new))
+                attn_out.append(ops.paged_attention(q, k, v, cache.block_table, cache.lens, batch.cu_new, ws, self.hq, self.hkv, batch.max_new,
+                                                    cache.timeout_ms))
             normed, h = self._reduce_norm(h, self.norm_mlp[l], attn_out, [w[l] for w in self.wo_run])
             act = [ops.silu_mul(gu) for gu in self._linear(normed, [w[l] for w in self.wgu], "gate_up")]
             gamma_next = self.norm_attn[l + 1] if l + 1 < cfg.layers else self.norm_final

@@ -63,6 +63,7 @@ class PagedCache:
         self.max_len = self.block_table.shape[1] * page
         need = load().paged_attention_workspace_bytes(model.hq // model.hkv, max(1, min(self.max_len, 1 << 20)), device)
         self.workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
+        self.timeout_ms = 2000  # of one wait inside the attention
 
     def extend(self, new_lens: torch.Tensor, rows: int, max_new: Optional[int] = None) -> PagedBatch:
         """Room for new_lens[i] more tokens of request i ([requests] int32 on the GPU); `rows` is the size of the batch that they are the first
