@@ -1,9 +1,10 @@
-"""Paged attention where infinities and NaN are in what the tokens see."""
+"""Paged attention where infinities and NaN are in what the tokens see, verification of probabilities that are NaN, and other streams than the
+tensors' own."""
 import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import D, assert_attention, attend, paged_problem
+from test_gpu_paged import D, attend, ints, ops, paged_problem
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +94,45 @@ def test_rows_that_see_nothing_are_zeros_whatever_the_values(hq, new):
     v[table[0][0], :, 0] = float("inf")
     out = attend((q, k, v, table, [1, total[1]], cu), hq, 1)
     assert (out[:new - 1] == 0).all()
+
+
+def test_verify_of_drafts_that_are_nan():
+    """A draft whose probability is NaN is turned down, and words of NaN have no weight behind it; where none has any, the target's own."""
+    nan = float("nan")
+    target = torch.tensor([[[0.25, 0.5, 0.25, 0], [1, 0, 0, 0.0]], [[0.25, 0.25, 0.5, 0], [1, 0, 0, 0.0]], [[0.0, 1, 0, 0], [1, 0, 0, 0.0]]], device="cuda")
+    draft = torch.tensor([[[0.5, nan, 0.1, 0.4]], [[0.1, nan, nan, 0.1]], [[nan] * 4]], device="cuda")
+    tokens, accept, sample = ints([[1]] * 3, torch.int64), torch.zeros(3, 1, device="cuda"), torch.full((3,), 0.5, device="cuda")
+    got = ops().verify_drafts(target, draft, tokens, None, accept, sample)
+    want = ref.verify(target.cpu(), draft.cpu(), tokens.cpu(), None, accept.cpu(), sample.cpu())
+    assert got[0].tolist() == want[0].tolist() == [[2, -1], [0, -1], [1, -1]] and got[1].tolist() == [0, 0, 0]
+
+
+def test_tables_append_and_verify_on_another_stream():
+    """What they read is made behind a pause on that stream: a call on another one would not see it."""
+    stream = torch.cuda.Stream()
+    lens, new, keep = ints([5, 0, 40]), ints([20, 3, 0]), ints([7, 0, 39])
+    table, free, n_free = ints([[0, -1], [-1, -1], [1, 2]]), ints([9, 8, 7, 6, 5, 4]), ints([3])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(23, 4 * D, device="cuda", generator=g).half()
+    k, v = (torch.zeros(10, 1, 32, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    target = torch.softmax(torch.randn(3, 3, 1000, device="cuda", generator=g), -1)
+    tokens, accept, sample = torch.randint(0, 1000, (3, 2), device="cuda", generator=g), torch.rand(3, 2, device="cuda", generator=g), torch.rand(3, device="cuda", generator=g)
+    torch.cuda.synchronize()
+
+    def calls():
+        n, ks, vs = new + 0, k.clone(), v.clone()
+        t, l, f, m = table.clone(), lens.clone(), free.clone(), n_free.clone()
+        cu, slots, positions, status = ops().paged_extend(t, l, n, f, m, 32, 23)
+        q = ops().rope_paged_append(x.mul(2), ks, vs, slots, positions, 2, 1, 1e4)
+        words = ops().verify_drafts(target.mul(1), None, tokens, None, accept, sample)
+        said = ops().paged_trim(t, l, keep, f, m, 32)
+        return [cu, slots, positions, status, q, ks, vs, *words, said, t, l, f, m]
+
+    want = [c.clone() for c in calls()]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(5_000_000)
+        got = calls()
+    stream.synchronize()
+    assert int(want[3]) == 0 and int(want[9]) == 0
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
