@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) paged_wide_kernel(const __gri
         ref = m;
       }
       if ((!split || w == 0) && busy) {
-        if (exists && !whole) *reinterpret_cast<float2*>(Piece<kWideRows>::slot(args, int(blockIdx.x), x->t0 > 0 ? 0 : 1) + 2 * (G0 + row)) = make_float2(ref, sum);
+        if (exists && !whole) *reinterpret_cast<float2*>(Piece<kWideRows>::slot(args, int(blockIdx.x), x->t0 > 0 ? 0 : 1) + 2 * (G0 + row)) = make_float2(sum == 0 && x->len - x->n + j >= 0 ? kNoWeight : ref, sum);
         float none = 0;  // for a row without a weight
         if (whole) {
           if (sum == 0) none = no_weight(x->len - x->n + j >= 0);

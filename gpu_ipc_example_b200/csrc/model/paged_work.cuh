@@ -254,7 +254,10 @@ __device__ __forceinline__ bool meet(bool leaving = false) {
   return all != 0;
 }
 
-// A piece: [rows] pairs (maximum in the log2 domain, sum), then [rows][128] of the output, not divided by the sum.
+// A piece: [rows] pairs (maximum in the log2 domain, sum), then [rows][128] of the output, not divided by the sum.  Where the sum is zero the wide
+// kernel's maximum is kNoWeight for a row that sees positions, all of whose scores here are -inf, and -inf for a row that sees none: the join
+// has that from the piece (from the lengths it would be a round to memory more, 2 us).
+constexpr float kNoWeight = -3.4028234663852886e38f;
 template <int ROWS>
 struct Piece {
   static constexpr size_t kFloats = size_t(ROWS) * (2 + kAttnD);
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   }
   auto write = [&](const Joined& x, int row) {
     const int at = next.row0 + row, j = at / a.group;
-    const float4 y = divided(x.o, x.l, next.r.len - next.r.n + j >= 0);
+    const float4 y = divided(x.o, x.l, x.m > -INFINITY);
     T* dst = static_cast<T*>(a.out) + (int64_t(next.r.row0 + j) * a.hq + int64_t(next.h) * a.group + (at - j * a.group)) * kAttnD + lane * 4;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
   };
