@@ -286,10 +286,11 @@ __device__ __forceinline__ float4 divided(const float4& o, float l, bool sees) {
 
 // ---- the join ---------------------------------------------------------------------------------------------------------
 // Where an item starts in span c = blockIdx.x and goes on in the next, its pieces are weighted with 2^(maximum - greatest maximum) and added
-// in order.  Eight rows a CTA: a warp each, or, where there are many pieces, all warps for one row after the other.
+// in order.  Eight rows a CTA, a warp each, whatever the pieces.  (All warps for one row after the other are as many rounds of loads behind one another,
+// and barriers besides: one request of 5 tokens x 8 heads at 32000, in 148 pieces, 37 us a call so, 26 with a warp each.)  Registers for four
+// pieces on their way at a time: with 32 a thread, which the compiler takes by itself, 28 us.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = kJoinThreads / 32;
-constexpr int kJoinMany = 24;  // pieces from which on the warps share a row: rounds of four loads, one after the other
 struct Joined {
   float m = -INFINITY, l = 0;
   float4 o = make_float4(0, 0, 0, 0);
@@ -302,9 +303,7 @@ struct Joined {
   }
 };
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int spans) {
-  __shared__ float2 s_ml[kJoinRows];
-  __shared__ __align__(16) float4 s_o[kJoinRows][32];
+__global__ void __launch_bounds__(kJoinThreads, 6) paged_join_kernel(const __grid_constant__ PagedArgs a, int spans) {
   pdl_launch_dependents();
   pdl_wait();
   const int c = int(blockIdx.x), warp = int(threadIdx.x >> 5), lane = int(threadIdx.x & 31);
@@ -319,37 +318,18 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     k += kJoinThreads;
     from = k <= spans ? a.starts[k] : Start{-1};
   }
-  auto write = [&](const Joined& x, int row) {
-    const int at = next.row0 + row, j = at / a.group;
-    const float4 y = divided(x.o, x.l, x.m > -INFINITY);
-    T* dst = static_cast<T*>(a.out) + (int64_t(next.r.row0 + j) * a.hq + int64_t(next.h) * a.group + (at - j * a.group)) * kAttnD + lane * 4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
-  };
-  auto gather = [&](int row, int first, int step) {
-    Joined x;
+  const int row = row0 + warp;
+  if (row >= next.rows) return;
+  Joined x;
 #pragma unroll 4
-    for (int n = first; n < pieces; n += step) {
-      const float* p = Piece<ROWS>::slot(a, c + n, n == 0 ? 1 : 0);
-      x.add(__ldcg(reinterpret_cast<const float2*>(p + 2 * row)), __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + size_t(row) * kAttnD + lane * 4)));
-    }
-    return x;
-  };
-  if (pieces < kJoinMany) {
-    if (row0 + warp < next.rows) write(gather(row0 + warp, 0, 1), row0 + warp);
-    return;
+  for (int n = 0; n < pieces; ++n) {
+    const float* p = Piece<ROWS>::slot(a, c + n, n == 0 ? 1 : 0);
+    x.add(__ldcg(reinterpret_cast<const float2*>(p + 2 * row)), __ldcg(reinterpret_cast<const float4*>(p + 2 * ROWS + size_t(row) * kAttnD + lane * 4)));
   }
-  for (int row = row0; row < min(row0 + kJoinRows, next.rows); ++row) {
-    const Joined mine = gather(row, warp, kJoinRows);
-    if (lane == 0) s_ml[warp] = make_float2(mine.m, mine.l);
-    s_o[warp][lane] = mine.o;
-    __syncthreads();
-    if (warp == (row & (kJoinRows - 1))) {
-      Joined x;
-      for (int w = 0; w < kJoinRows; ++w) x.add(s_ml[w], s_o[w][lane]);
-      write(x, row);
-    }
-    __syncthreads();
-  }
+  const int at = next.row0 + row, j = at / a.group;
+  const float4 y = divided(x.o, x.l, x.m > -INFINITY);
+  T* dst = static_cast<T*>(a.out) + (int64_t(next.r.row0 + j) * a.hq + int64_t(next.h) * a.group + (at - j * a.group)) * kAttnD + lane * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
 }
 
 }  // namespace b200ipc
