@@ -370,7 +370,8 @@ class LlamaTP:
             if draft_lens is not None:
                 hidden = [x[at.clamp(max=rows - 1)] for x in hidden]
             probs = self.probabilities(hidden, temperature).view(B, K + 1, -1)
-            tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts.contiguous(), draft_lens, accept.contiguous(), sample.contiguous())
+            lens = None if draft_lens is None else draft_lens.contiguous()
+            tokens, accepted = torch.ops.b200ipc.verify_drafts(probs, draft_probs, drafts.contiguous(), lens, accept.contiguous(), sample.contiguous())
             made = batch.cu_new[1:] > batch.cu_new[:-1]
             tokens, accepted = tokens.masked_fill_(~made[:, None], -1), accepted.masked_fill_(~made, -1)
             keep = torch.minimum(cache.lens, before + accepted + 1)
