@@ -6,7 +6,7 @@
 //
 // Bound by memory: (hq + 2 hkv) x 256 bytes in and out per token.  One CTA per token: 16-byte loads and stores, eight pairs a thread
 // (two vectors 64 elements apart), the loads of a thread's first heads in flight while the angles are computed.  4001 tokens of
-// 64 + 2 x 8 heads, 167 MB in and out: 28.5 us, 5.9 TB/s; 32 tokens: 2.3 us in a graph.
+// 64 + 2 x 8 heads, 167 MB in and out: 28.5 us, 5.9 TB/s; 32 tokens: 1.9 us in a graph.
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "decode_math.cuh"

@@ -58,7 +58,7 @@ template <typename T>
 void run(PagedArgs& a, const PagedAttentionShape& s, char* workspace, int spans, cudaStream_t stream) {
   void* params[] = {&a, &spans};
   // Up to 16 rows for every request: the narrow kernel.  A batch with longer ones is the wide kernel's as a whole, which for single tokens alone is
-  // behind by 6 us a call and 10 % (32 x 2048 15.1 and 20.7 us, 16 x 32768 53.2 and 60.4), but has them read while it computes for
+  // behind by 7 us a call (32 x 2048 15.5 and 22.8 us, 16 x 32768 53.1 and 59.6), but has them read while it computes for
   // the others (a chunk of 2047 tokens among 23 requests 170 us with both kernels, 147 with this one).
   const int64_t most = int64_t(s.max_new) * a.group;
   if (most <= kNarRows) {

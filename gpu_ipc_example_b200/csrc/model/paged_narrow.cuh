@@ -9,7 +9,7 @@
 // must come from who has seen the round before, as copies may land out of order), 16 positions of a tile each.  Scores, maxima, sums
 // and outputs are fp32; the weights are rounded to 16 bits for the second product, as the tensor cores take them.
 //
-// 16 requests of up to 32768 tokens, two KV heads: 290 MB in 53.2 us, 5.4 TB/s over the launch; 32 of 2048, one KV head: 33.7 MB in 15.1 us, of which
+// 16 requests of up to 32768 tokens, two KV heads: 290 MB in 53 us, 5.4 TB/s over the launch; 32 of 2048, one KV head: 33.7 MB in 15.5 us, of which
 // 5.1 would be memory's: 4 pass until the first tile is there (lengths, span, table, copy, each a round to memory behind the other), 3 at
 // the end (pieces out, the last CTA's reads, its rows out).
 #pragma once

@@ -4,8 +4,8 @@
 // out: the call is bound by latency (launch, one round of loads, the scan, one round of stores), so one kernel does it all.  Every CTA
 // of one cluster makes the same scan of all requests in its shared memory and then takes a share of the pages and tokens, whose request
 // it finds by bisection.  The lengths are written in place, so a CTA writes only when all have read (the cluster's barrier), which is
-// also why it is one cluster and not a grid.  Extend and trim of 32 requests by a token 6.0 us, of 512 requests by up to 64 tokens 11.8
-// (in a graph); a call by itself takes 6 of host time.
+// also why it is one cluster and not a grid.  Extend and trim of 32 requests by a token 5.8 us, of 512 requests by up to 64 tokens 11.7
+// (in a graph); a call by itself takes 8 (extend, four outputs) and 6.5 (trim) of host time.
 #include <climits>
 
 #include "../common/check.h"

@@ -22,11 +22,13 @@
 // The running maximum is only moved when it grows by more than 2^8: till then weights are up to 256 instead of 1, which fp32 sums and
 // 16-bit weights hold alike (relative rounding), and O is left alone.
 //
-// Where rows are many it is bound by shared memory and the softmax alike: a pair of accumulators over a tile reads 192 KB for the scores (both
-// operands, Q again for every 64 positions) and 64 for the outputs, and TMA writes 64: 2560 clocks at 128 bytes each; the weights are
-// 2048 clocks of exponentials, three quarters of them left.  (Prompts, 396 us: 371 without the softmax's arithmetic, 359 with an eighth of
-// the products, 249 with neither.)  Where they are few, by memory and the way from one item to the next.  Prompts of up to 4096 tokens,
-// 397 GFLOP: 395 us, 1005 TFLOP/s (460 - 475 us under the power cap); a chunk of 512 tokens at 16384, 34.9 GFLOP: 48 us, 8 of them the join of
+// Where rows are many no one unit bounds it.  A pair of accumulators over a tile is 2048 clocks of tensor cores, 2560 of shared memory (192 KB
+// read for the scores, Q again for every 64 positions, 64 for the outputs, 64 written by TMA, at 128 bytes each) and 1536 of exponentials (2048, a
+// quarter of them by polynomial), and about 4100 pass.  Prompts, 396 us when it was measured: 371 without the softmax's arithmetic, 359 with an
+// eighth of the products, 249 with neither; so the greater part is the way between the two, arrivals, waits, loads and stores of tensor
+// memory and issue, twice a tile as scores come by halves.  One buffer of 128 positions an accumulator whose weights are handed over in
+// parts has not been tried.  Where rows are few, it is bound by memory and the way from one item to the next.  Prompts of up to 4096 tokens, 397 GFLOP:
+// 393 us, 1010 TFLOP/s (435 - 475 us under the power cap); a chunk of 512 tokens at 16384, 34.9 GFLOP: 47.6 us, 8 of them the join of
 // pieces; 24 requests of 5 tokens, 103 MB: 32 us; a chunk of 2047 tokens among 23 single ones, 107 GFLOP and 234 MB: 146 us.
 #pragma once
 

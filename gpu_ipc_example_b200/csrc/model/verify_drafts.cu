@@ -12,8 +12,9 @@
 // Bound by memory: of all the rows one of p and one of q is read, 8 bytes a word.  A request is a cluster of CTAs, each with a piece of
 // the vocabulary, each of its warps with a run of it; the sums of all warps are exchanged through distributed shared memory, every CTA
 // adds them in the same order, and the one warp whose run holds the sampled place reads that run again (from L1 or L2).  32 requests,
-// four drafts, 128256 words: 10.9 us, of which 21.6 MB of memory traffic are 3.3; the rest is a chain of launch, gathers of the drafts' words,
-// the stream's first arrival, the exchange and the second reading.  With loads that the compiler issued one round at a time it was 15.
+// four drafts, 128256 words: 10.9 us (10.2 without the drafts' probabilities; of 32000 words 7.4 and 7.1), of which 21.6 MB of memory traffic are
+// 3.3; the rest is a chain of launch, gathers of the drafts' words, the stream's first arrival, the exchange and the second reading.  With
+// loads that the compiler issued one round at a time it was 15.
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "paged_ops.h"
