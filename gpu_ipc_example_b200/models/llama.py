@@ -284,8 +284,8 @@ class LlamaTP:
         whole prompts, chunks of them, single tokens and drafts alike.  Returns the final-norm output [rows, hidden] of every local rank.
         Rows without a token are computed like the others and mean nothing.
 
-        A serving loop that captures steps, or that uses fusion="gemm" (whose outputs are kept by shape), takes few different
-        numbers of rows and leaves the last ones empty."""
+        A serving loop that captures steps, or that uses fusion="gemm" (whose outputs are kept by shape, so that hidden states have to be used or
+        copied before the next step of as many rows), takes few different numbers of rows and leaves the last ones empty."""
         cfg = self.cfg
         if not self.kernels:
             raise ValueError("forward_paged is for the decode kernels")

@@ -127,6 +127,27 @@ def test_requests_with_fewer_drafts_and_without_any_part(certain):
         assert int(cache.n_free) == 20 - sum(ref.pages_of(n, 16) for n in cache.lens.tolist())
 
 
+@pytest.mark.parametrize("world,fusion", [(1, "gemm"), (2, "gemm"), (2, "allreduce")])
+def test_steps_without_drafts_and_without_requests(world, fusion):
+    """No drafts at all: a word is drawn for every request.  No request that takes part: nothing happens.  Numbers outside of -1 .. K are cut off."""
+    with Communicator.virtual(world, 0, staging_bytes=64 << 20) as comm:
+        model = LlamaTP(LlamaConfig.tiny128(), comm, batch=1, max_ctx=8, fusion=fusion, seed=4)
+        cache = PagedCache(model, requests=3, max_len=64, pages=20, page=16)
+        g = torch.Generator(device="cuda").manual_seed(8)
+        served(model, [torch.randint(0, model.cfg.vocab, (n,), device="cuda", generator=g) for n in (5, 1, 20)], [[5], [1], [20]], cache)
+        last, drafts, probs, accept, sample = numbers(model, 3, g)
+        before = tables(cache)
+        tokens, accepted = model.verify(last, drafts, probs, cache, accept, sample, draft_lens=ints([-1, -1, -1]))
+        assert (tokens == -1).all() and (accepted == -1).all() and all(torch.equal(a, b) for a, b in zip(before, tables(cache)))
+        tokens, accepted = model.verify(last, drafts[:, :0], None, cache, accept[:, :0], sample)
+        assert accepted.tolist() == [0] * 3 and all(0 <= t < model.cfg.vocab for t in tokens[:, 0].tolist()) and cache.lens.tolist() == [6, 2, 21]
+        tokens, accepted = model.verify(last, drafts, None, cache, torch.zeros_like(accept), sample, draft_lens=ints([-7, 99, 1]))
+        assert accepted.tolist() == [-1, K, 1] and cache.lens.tolist() == [6, 2 + K + 1, 23]
+        assert tokens[1, :K].tolist() == drafts[1].tolist() and tokens[0].tolist() == [-1] * (K + 1)
+        cache.check()
+        comm.check()
+
+
 def test_a_captured_speculative_step():
     """Draft lengths change between the replays, and the pages run out in the end."""
     with Communicator.virtual(1, 0, staging_bytes=16 << 20) as comm:
